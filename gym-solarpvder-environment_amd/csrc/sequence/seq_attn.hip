@@ -100,7 +100,8 @@ __device__ __forceinline__ bool whose(const Args &A, long long &grp, int &sib) {
     return grp < A.n_groups;
 }
 
-template <typename T, int DKP, int DVS, bool STATE_ONLY>
+// WHOLE: heads of exactly DKP and a multiple of DVS
+template <typename T, int DKP, int DVS, bool WHOLE, bool STATE_ONLY>
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(DKP * DVS > 4096 ? 1 : 2)))
 void seq_scan_kernel(const Args A) {
     typedef Ty<T> Y;
@@ -196,91 +197,126 @@ void seq_scan_kernel(const Args A) {
         gn = power(lg, n);
     };
 
-    // ---- loads of a chunk [a, a + n): rows at and behind n are zeros
+    // ---- loads of a chunk [a, a + n), raw: rows behind n and pieces behind the head's end are read from places that exist, and put
+    // right by `mend` when they are used.  Offsets of a lane are 32-bit, from a base that the wave shares.
     frag nq[NT][KS], nk[TT][KS], nv[TT][VS];
-    unsigned long long nmask = 0;
-    auto load = [&](int a, int n) {
+    const unsigned q_t = (unsigned)(S.q_t * sizeof(T)), k_t = (unsigned)(S.k_t * sizeof(T)), v_t = (unsigned)(S.v_t * sizeof(T));
+    const unsigned in_row = V * g * sizeof(T);
+    unsigned qo[NT], ko[TT], vo[TT];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int x = 16 * nt + m;
+    for (int nt = 0; nt < NT; ++nt) qo[nt] = (16 * nt + m) * q_t;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                if (!STATE_ONLY) nq[nt][ks] = load_row<T>(Q + (long long)(a + x) * S.q_t, ks * Y::KW + V * g, x < n ? DK : 0);
-            }
+    for (int t = 0; t < TT; ++t) { ko[t] = Y::tile_row(t, m) * k_t; vo[t] = Y::tile_row(t, m) * v_t; }
+    auto piece = [&](const char *base, unsigned row, int p, int dim) {
+        frag f;
+        if constexpr (WHOLE) {
+            __builtin_memcpy(&f, base + (row + in_row) + p * (int)(Y::KW * sizeof(T)), 16);
+        } else if (dim >= V) {
+            const int d = p * Y::KW + V * g, last = dim - V;
+            __builtin_memcpy(&f, base + (row + (unsigned)((d < last ? d : last) * sizeof(T))), 16);
+        } else {                                            // heads of a few elements
+            const T *r = (const T *)(base + row);
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = r[e < dim ? e : 0];
         }
+        return f;
+    };
+    auto mend = [&](frag &f, bool row_is, int p, int dim) {
+        if constexpr (!WHOLE) {
+            const int d = p * Y::KW + V * g, last = dim - V;
+            if (dim % V != 0) {
+                if (dim >= V) f = behind(f, d > last ? d - last : 0);
+                else
+#pragma unroll
+                    for (int e = 0; e < V; ++e) f[e] = d + e < dim ? f[e] : (T)0.f;
+            }
+            row_is = row_is && d < dim;
+        }
+        const u4 u = __builtin_bit_cast(u4, f);
+        f = __builtin_bit_cast(frag, row_is ? u : u4{0u, 0u, 0u, 0u});
+    };
+    auto load_q = [&](int a, int n) {
+        if constexpr (!STATE_ONLY) {
+            const char *base = (const char *)(Q + (long long)a * S.q_t);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) nq[nt][ks] = piece(base, 16 * nt + m < n ? qo[nt] : 0u, ks, DK);
+        }
+    };
+    auto load_kv = [&](int a, int n) {
+        const char *kb = (const char *)(K + (long long)a * S.k_t), *vb = (const char *)(Vp + (long long)a * S.v_t);
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
-            const int y = Y::tile_row(t, m);
+            const bool is = Y::tile_row(t, m) < n;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) nk[t][ks] = load_row<T>(K + (long long)(a + y) * S.k_t, ks * Y::KW + V * g, y < n ? DK : 0);
+            for (int ks = 0; ks < KS; ++ks) nk[t][ks] = piece(kb, is ? ko[t] : 0u, ks, DK);
 #pragma unroll
-            for (int vs = 0; vs < VS; ++vs) nv[t][vs] = load_row<T>(Vp + (long long)(a + y) * S.v_t, vs * Y::KW + V * g, y < n ? DV : 0);
+            for (int vs = 0; vs < VS; ++vs) nv[t][vs] = piece(vb, is ? vo[t] : 0u, vs, DV);
         }
-        nmask = 0;
-        if (St) nmask = __ballot(lane < n && St[(long long)(a + lane) * A.a.starts_t] != 0);
     };
+    auto mend_all = [&](int n) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            if constexpr (!STATE_ONLY) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mend(nq[nt][ks], 16 * nt + m < n, ks, DK);
+            }
+#pragma unroll
+            for (int t = 0; t < TT; ++t) mend(nk[t][ks], Y::tile_row(t, m) < n, ks, DK);
+        }
+#pragma unroll
+        for (int vs = 0; vs < VS; ++vs)
+#pragma unroll
+            for (int t = 0; t < TT; ++t) mend(nv[t][vs], Y::tile_row(t, m) < n, vs, DV);
+    };
+    uint8_t nflag = 0;
+    auto load_flags = [&](int a, int n) { nflag = St && lane < n ? St[(long long)(a + lane) * A.a.starts_t] : 0; };
 
     bool any_start = false;
-    int pos = rev ? tok_e : tok_a;
-    auto left = [&]() { return rev ? pos - tok_a : tok_e - pos; };
-    int n = left() < C ? left() : C;
-    if (n > 0) load(rev ? pos - n : pos, n);
+    int pos = rev ? tok_e : tok_a, most = C;
+    auto left = [&]() { const int l = rev ? pos - tok_a : tok_e - pos; return l < most ? l : most; };
+    int n = left();
+    if (n > 0) { const int a = rev ? pos - n : pos; load_kv(a, n); load_q(a, n); load_flags(a, n); }
     while (n > 0) {
-        // A value that is not finite would reach other tokens through a weight of zero (0 x NaN).  Such a chunk is taken token by
-        // token instead, where no token shares a product with another.  The check sums the operands on the matrix cores.
-        bool bad = false;
-        if (n > 1) {
-            if constexpr (Y::TT == 2) {
-                f4 z0 = {0.f, 0.f, 0.f, 0.f}, z1 = z0;
-                frag one;
-#pragma unroll
-                for (int e = 0; e < V; ++e) one[e] = (T)1.f;
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) { z0 = Y::mfma(one, nk[0][ks], z0); z1 = Y::mfma(one, nk[1][ks], z1); }
-#pragma unroll
-                for (int vs = 0; vs < VS; ++vs) { z0 = Y::mfma(one, nv[0][vs], z0); z1 = Y::mfma(one, nv[1][vs], z1); }
-                const float z = z0[0] * 0.f + z1[0] * 0.f;
-                bad = __any(z != 0.f || z != z);
-            } else {
-                float z = 0.f;
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-#pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) z = __builtin_fmaf((float)nk[0][ks][e], 0.f, z);
-#pragma unroll
-                    for (int vs = 0; vs < VS; ++vs) z = __builtin_fmaf((float)nv[0][vs][e], 0.f, z);
-                }
-                bad = __any(z != 0.f || z != z);
-            }
-            if (bad) { n = 1; load(rev ? pos - 1 : pos, 1); }
-        }
         by_length(n);
-        const int a = rev ? pos - n : pos;
-        const unsigned mask = (unsigned)nmask;
-        frag q[NT][KS], k[TT][KS];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) q[nt][ks] = nq[nt][ks];
+        const int a = rev ? pos - n : pos, pos0 = pos;
+        const unsigned mask = St ? (unsigned)__ballot(nflag != 0) : 0u;
+        // (the starts of a chunk as bits: x and y are of one episode if no bit lies behind the earlier and up to the later)
+        const unsigned upto_last = (2u << (n - 1)) - 1u;
+        if (!WHOLE || n < C) mend_all(n);
         wave_sync();                                     // the chunk before has been read
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
             const int y = Y::tile_row(t, m);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                k[t][ks] = nk[t][ks];
-                *(frag *)(ldsK + y * (DKP + Y::PAD) + ks * Y::KW + V * g) = nk[t][ks];
-            }
+            for (int ks = 0; ks < KS; ++ks) *(frag *)(ldsK + y * (DKP + Y::PAD) + ks * Y::KW + V * g) = nk[t][ks];
 #pragma unroll
             for (int vs = 0; vs < VS; ++vs) *(frag *)(ldsV + y * (DVS + Y::PAD) + vs * Y::KW + V * g) = nv[t][vs];
         }
         wave_sync();
-        pos += rev ? -n : n;
-        const int n2 = left() < C ? left() : C;
-        if (n2 > 0) load(rev ? pos - n2 : pos, n2);      // in flight while this chunk is computed
-
-        // (the starts of a chunk as bits: x and y are of one episode if no bit lies behind the earlier and up to the later)
-        const unsigned upto_last = (2u << (n - 1)) - 1u;
+        // A value that is not finite would reach other tokens through a weight of zero (0 x NaN).  Such a chunk is taken token by
+        // token instead, where no token shares a product with another.  The check sums the operands on the matrix cores.
+        float z = 0.f;
+        if constexpr (TT == 2) {
+            f4 z0 = {0.f, 0.f, 0.f, 0.f}, z1 = z0;
+            frag one;
+#pragma unroll
+            for (int e = 0; e < V; ++e) one[e] = (T)1.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) { z0 = Y::mfma(one, nk[0][ks], z0); z1 = Y::mfma(one, nk[1][ks], z1); }
+#pragma unroll
+            for (int vs = 0; vs < VS; ++vs) { z0 = Y::mfma(one, nv[0][vs], z0); z1 = Y::mfma(one, nv[1][vs], z1); }
+            z = z0[0] * 0.f + z1[0] * 0.f;
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) z = __builtin_fmaf((float)nk[0][ks][e], 0.f, z);
+#pragma unroll
+                for (int vs = 0; vs < VS; ++vs) z = __builtin_fmaf((float)nv[0][vs][e], 0.f, z);
+            }
+        }
         frag p[NT];
         if constexpr (!STATE_ONLY) {
 #pragma unroll
@@ -290,17 +326,16 @@ void seq_scan_kernel(const Args A) {
                 for (int t = 0; t < TT; ++t) {
                     at[t] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) at[t] = Y::mfma(k[t][ks], q[nt][ks], at[t]);
+                    for (int ks = 0; ks < KS; ++ks) at[t] = Y::mfma(nk[t][ks], nq[nt][ks], at[t]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int x = 16 * nt + m, y = V * g + 4 * t + r;
-                        const float w = dw[nt][t][r], v = at[t][r] * w;
-                        bool see = rev ? y >= x : y <= x;             // (a weight of zero does not clear an infinite product)
+                        float w = dw[nt][t][r];
                         if (mask) {
+                            const int x = 16 * nt + m, y = V * g + 4 * t + r;
                             const unsigned bits = ((2u << x) - 1u) ^ ((2u << y) - 1u);   // the tokens behind one, up to the other
-                            see = see && (mask & bits) == 0;
+                            w = (mask & bits) == 0 ? w : 0.f;
                         }
-                        at[t][r] = see ? v : 0.f;
+                        at[t][r] = mul_or_zero(at[t][r], w);
                     }
                 }
                 p[nt] = Y::operand(at);
@@ -308,43 +343,68 @@ void seq_scan_kernel(const Args A) {
         }
         frag vf[NJ];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) vf[j] = Y::template column<DVS>(ldsV, Y::KW * (j / TT), j % TT, m, g) ;
+        for (int j = 0; j < NJ; ++j) vf[j] = Y::template column<DVS>(ldsV, Y::KW * (j / TT), j % TT, m, g);
+        // the next chunk's loads are in flight while this one is computed
+        pos += rev ? -n : n;
+        most = C;
+        const int n2 = left(), a2 = rev ? pos - n2 : pos;
+        if (n2 > 0) load_kv(a2, n2);
+        f4 o[VS][NT][TT];
         if constexpr (!STATE_ONLY) {
-            // P and S as operands are rounded to the inputs' type: 2^-9 of each term at bf16, half of what the output's own rounding
-            // allows over many terms; the sums are fp32
+            // P and S as operands are rounded to the inputs' type: 2^-9 of each term at bf16, as much as the output's own rounding; the
+            // sums are fp32
 #pragma unroll
-            for (int jg = 0; jg < VS; ++jg) {
-                f4 o[NT][TT];
+            for (int j = 0; j < NJ; ++j) {
 #pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    const int j = jg * TT + t;
+                for (int nt = 0; nt < NT; ++nt) o[j / TT][nt][j % TT] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) o[nt][t] = f4{0.f, 0.f, 0.f, 0.f};
+                for (int ks = 0; ks < KS; ++ks) {
+                    f4 rows[TT];
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        f4 rows[TT];
+                    for (int tt = 0; tt < TT; ++tt) rows[tt] = s[ks * TT + tt][j];
+                    const frag sf = Y::operand(rows);
 #pragma unroll
-                        for (int tt = 0; tt < TT; ++tt) rows[tt] = s[ks * TT + tt][j];
-                        const frag sf = Y::operand(rows);
+                    for (int nt = 0; nt < NT; ++nt) o[j / TT][nt][j % TT] = Y::mfma(sf, nq[nt][ks], o[j / TT][nt][j % TT]);
+                }
+            }
+        }
+        if (n2 > 0) { load_q(a2, n2); load_flags(a2, n2); }
+        if constexpr (!STATE_ONLY) {
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) o[nt][t] = Y::mfma(sf, q[nt][ks], o[nt][t]);
-                    }
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        bool reach = true;
-                        if (mask) {
-                            const int x = 16 * nt + m;
-                            const unsigned upto = (2u << x) - 1u;
-                            reach = (rev ? mask & upto_last & ~upto : mask & upto) == 0;
-                        }
-                        o[nt][t] = reach ? o[nt][t] * rx[nt] : f4{0.f, 0.f, 0.f, 0.f};
-                        o[nt][t] = Y::mfma(vf[j], p[nt], o[nt][t]);
-                    }
+            for (int nt = 0; nt < NT; ++nt) {
+                float reach = rx[nt];
+                if (mask) {
+                    const unsigned upto = (2u << (16 * nt + m)) - 1u;
+                    reach = (rev ? mask & upto_last & ~upto : mask & upto) == 0 ? reach : 0.f;
                 }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const int x = 16 * nt + m;
-                    if (x < n) store_row<T>(O + (long long)(a + x) * S.o_t, jg * Y::KW + V * g, DV, Y::operand(o[nt]));
+                for (int j = 0; j < NJ; ++j) {
+                    f4 &t = o[j / TT][nt][j % TT];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) t[r] = mul_or_zero(t[r], reach);
+                    t = Y::mfma(vf[j], p[nt], t);
+                }
+            }
+        }
+        if (n > 1 && __any(z != 0.f || z != z)) {
+            pos = pos0;
+            most = n = 1;
+            const int a1 = rev ? pos - 1 : pos;
+            load_kv(a1, 1); load_q(a1, 1); load_flags(a1, 1);
+            continue;
+        }
+        if constexpr (!STATE_ONLY) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int x = 16 * nt + m;
+                if (x < n) {
+                    T *row = O + (long long)(a + x) * S.o_t;
+#pragma unroll
+                    for (int jg = 0; jg < VS; ++jg) {
+                        const frag f = Y::operand(o[jg][nt]);
+                        if constexpr (WHOLE) __builtin_memcpy(row + jg * Y::KW + V * g, &f, 16);
+                        else store_row<T>(row, jg * Y::KW + V * g, DV, f);
+                    }
                 }
             }
         }
@@ -354,17 +414,19 @@ void seq_scan_kernel(const Args A) {
         for (int e = 0; e < V; ++e) {
             w[e] = wy[e];
             if (mask) {
-                const int y = V * g + e;
-                const unsigned upto = (2u << (y & 31)) - 1u;
+                const unsigned upto = (2u << ((V * g + e) & 31)) - 1u;
                 if ((rev ? mask & upto : mask & upto_last & ~upto) != 0) w[e] = 0.f;
             }
         }
         const bool fresh = (mask & upto_last) != 0;
         any_start = any_start || fresh;
+        const float gs = fresh ? 0.f : gn;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) s[i][j] = fresh ? f4{0.f, 0.f, 0.f, 0.f} : s[i][j] * gn;
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[i][j][r] = mul_or_zero(s[i][j][r], gs);
         frag kt[NI];
 #pragma unroll
         for (int i = 0; i < NI; ++i) kt[i] = Y::template column<DKP>(ldsK, Y::KW * (i / TT), i % TT, m, g);
@@ -485,23 +547,29 @@ int seg_len_of(const pvder_seq_attn *a) {
     return (per + c - 1) / c * c;
 }
 
-template <typename T, int DKP, int DVS> int launch(const Args &A, hipStream_t st) {
+template <typename T, int DKP, int DVS, bool WHOLE> int launch(const Args &A, hipStream_t st) {
     const long long blocks = (A.n_groups + 7) / 8 * 8 * A.n_sib;
     if (blocks > 0x7fffffffll) return kEinval;
     if (A.a.segments > 1) {
-        seq_scan_kernel<T, DKP, DVS, true><<<dim3((unsigned)blocks), dim3(64), 0, st>>>(A);
+        seq_scan_kernel<T, DKP, DVS, WHOLE, true><<<dim3((unsigned)blocks), dim3(64), 0, st>>>(A);
         const long long items = (long long)A.a.B * A.a.H * A.n_sib * (DKP * DVS / 4);
         seq_join_kernel<T, DKP, DVS><<<dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st>>>(A);
     }
-    seq_scan_kernel<T, DKP, DVS, false><<<dim3((unsigned)blocks), dim3(64), 0, st>>>(A);
+    seq_scan_kernel<T, DKP, DVS, WHOLE, false><<<dim3((unsigned)blocks), dim3(64), 0, st>>>(A);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : -(int)e;
 }
 
+template <typename T, int DKP, int DVS> int fit(const Args &A, hipStream_t st) {
+    bool whole = true;
+    for (int i = 0; i < A.a.n_scans; ++i) whole = whole && A.a.scan[i].dk == DKP && A.a.scan[i].dv % DVS == 0;
+    return whole ? launch<T, DKP, DVS, true>(A, st) : launch<T, DKP, DVS, false>(A, st);
+}
+
 template <typename T> int pick(const Args &A, const Plan &P, hipStream_t st) {
-    if (P.dkp == 32) return P.dvs == 32 ? launch<T, 32, 32>(A, st) : launch<T, 32, 64>(A, st);
-    if (P.dkp == 64) return P.dvs == 32 ? launch<T, 64, 32>(A, st) : launch<T, 64, 64>(A, st);
-    return launch<T, 128, 32>(A, st);
+    if (P.dkp == 32) return P.dvs == 32 ? fit<T, 32, 32>(A, st) : fit<T, 32, 64>(A, st);
+    if (P.dkp == 64) return P.dvs == 32 ? fit<T, 64, 32>(A, st) : fit<T, 64, 64>(A, st);
+    return fit<T, 128, 32>(A, st);
 }
 
 }  // namespace
@@ -528,7 +596,12 @@ extern "C" int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream) {
     if (a->segments > 1 && (!a->workspace || ((uintptr_t)a->workspace & 15))) return kEinval;
     if (a->B > 0 && a->T > 0)
         for (int i = 0; i < a->n_scans; ++i)
-            if (!a->scan[i].q || !a->scan[i].k || !a->scan[i].v || !a->scan[i].o) return kEinval;
+        {
+            const pvder_seq_scan &s = a->scan[i];
+            if (!s.q || !s.k || !s.v || !s.o) return kEinval;
+            const int64_t most = PVDER_SEQ_MAX_TOKEN_STRIDE / (a->dtype == PVDER_SEQ_BF16 ? 2 : 4);
+            if (s.q_t < 0 || s.k_t < 0 || s.v_t < 0 || s.q_t > most || s.k_t > most || s.v_t > most) return kEinval;
+        }
     if (a->B == 0) return 0;
     A.a = *a;
     if (A.a.T == 0) A.a.segments = 1;

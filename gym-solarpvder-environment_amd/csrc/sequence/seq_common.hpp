@@ -20,15 +20,36 @@ template <typename T> struct Vec;
 template <> struct Vec<float> { typedef f4 type; static constexpr int N = 4; };
 template <> struct Vec<__bf16> { typedef b8 type; static constexpr int N = 8; };
 
+// f's elements from `n` on, in the first places; zeros behind them (n >= 0)
+__device__ __forceinline__ f4 behind(f4 f, int n) {
+    u4 u = __builtin_bit_cast(u4, f);
+    if (n & 2) u = u4{u.z, u.w, 0u, 0u};
+    if (n & 1) u = u4{u.y, u.z, u.w, 0u};
+    if (n >= 4) u = u4{0u, 0u, 0u, 0u};
+    return __builtin_bit_cast(f4, u);
+}
+__device__ __forceinline__ b8 behind(b8 f, int n) {
+    u4 u = __builtin_bit_cast(u4, f);
+    if (n & 4) u = u4{u.z, u.w, 0u, 0u};
+    if (n & 2) u = u4{u.y, u.z, u.w, 0u};
+    if (n & 1) u = u4{(u.x >> 16) | (u.y << 16), (u.y >> 16) | (u.z << 16), (u.z >> 16) | (u.w << 16), u.w >> 16};
+    if (n >= 8) u = u4{0u, 0u, 0u, 0u};
+    return __builtin_bit_cast(b8, u);
+}
+
 // 16 bytes of a row from element d on; elements at and behind `dim` are zeros and not read.  No alignment is asked of the row.
-template <typename T> __device__ __forceinline__ typename Vec<T>::type load_row(const T *row, int d, int dim) {
+// Rows of 16 bytes and more take one load whatever d is (the piece that the row's end cuts is read from 16 bytes before that end and
+// shifted), so that loads of many rows are in flight together; a row behind the last (`ok` false) has to be readable all the same.
+template <typename T> __device__ __forceinline__ typename Vec<T>::type load_row(const T *row, int d, int dim, bool ok = true) {
     constexpr int V = Vec<T>::N;
     typename Vec<T>::type f;
-    if (d + V <= dim) {
-        __builtin_memcpy(&f, row + d, 16);
+    if (dim >= V) {
+        const int last = dim - V, at = d < last ? d : last;
+        __builtin_memcpy(&f, row + at, 16);
+        f = behind(f, ok ? d - at : V);
     } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = d + e < dim ? row[d + e] : (T)0.f;
+        for (int e = 0; e < V; ++e) f[e] = ok && d + e < dim ? row[d + e] : (T)0.f;
     }
     return f;
 }
@@ -42,6 +63,10 @@ template <typename T> __device__ __forceinline__ void store_row(T *row, int d, i
             if (d + e < dim) row[d + e] = f[e];
     }
 }
+
+// a * b, and 0 where b is 0 whatever a is (NaN and infinities too)
+extern "C" __device__ float pvder_seq_mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
+__device__ __forceinline__ float mul_or_zero(float a, float b) { return pvder_seq_mul_legacy(a, b); }
 
 // g^n of a decay given as its base-2 logarithm lg <= 0; g^0 = 1 also where lg is -infinity
 __device__ __forceinline__ float power(float lg, int n) { return n == 0 ? 1.f : exp2f(lg * (float)n); }

@@ -24,7 +24,7 @@ import torch
 
 from .. import _native
 
-MAX_HEAD, MAX_WIDTH = 128, 8192                      # include/pvder_sequence.h
+MAX_HEAD, MAX_WIDTH, MAX_TOKEN_STRIDE = 128, 8192, 1 << 26     # include/pvder_sequence.h
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 # struct pvder_seq_scan, pvder_seq_attn, pvder_seq_step, pvder_seq_norm
@@ -60,6 +60,12 @@ def _on(device: torch.device):
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` with unit stride in its last dimension (a copy only where it has another)."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _tokens(t: torch.Tensor) -> torch.Tensor:
+    """``_rows`` of a [B, T, H, D] tensor whose tokens lie near enough for the kernels' 32-bit offsets within a chunk."""
+    t = _rows(t)
+    return t if t.stride(1) * t.element_size() <= MAX_TOKEN_STRIDE else t.contiguous()
 
 
 def _tensors(device: Optional[torch.device], **tensors) -> torch.device:
@@ -175,7 +181,7 @@ class _DecayAttention(torch.autograd.Function):
         if dout is None and dfinal is None:
             return none
         dev, dt = q.device, q.dtype
-        dout = torch.zeros((B, T, H, DV), dtype=dt, device=dev) if dout is None else _rows(dout)
+        dout = torch.zeros((B, T, H, DV), dtype=dt, device=dev) if dout is None else _tokens(dout)
         if dfinal is not None and not dfinal.is_contiguous():
             dfinal = dfinal.contiguous()
         need_q, need_k, need_v, _, need_s = ctx.needs_input_grad[:5]
@@ -238,7 +244,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
             _need(lengths.shape == (B,) and lengths.is_contiguous(), "lengths must be a contiguous [%d]" % B)
     scale = _scale(scale, DK)
     _gpu("q", q)
-    q, k, v = _rows(q), _rows(k), _rows(v)
+    q, k, v = _tokens(q), _tokens(k), _tokens(v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (initial_state is not None and initial_state.requires_grad)):
         return _DecayAttention.apply(q, k, v, log_decay, initial_state, starts, lengths, scale, bool(output_final_state))

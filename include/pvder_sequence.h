@@ -14,7 +14,7 @@ extern "C" {
 #endif
 
 enum { PVDER_SEQ_F32 = 0, PVDER_SEQ_BF16 = 1 };
-enum { PVDER_SEQ_MAX_HEAD = 128, PVDER_SEQ_MAX_SCANS = 3, PVDER_SEQ_MAX_WIDTH = 8192 };
+enum { PVDER_SEQ_MAX_HEAD = 128, PVDER_SEQ_MAX_SCANS = 3, PVDER_SEQ_MAX_WIDTH = 8192, PVDER_SEQ_MAX_TOKEN_STRIDE = 1 << 26 };
 
 /* One scan over the tokens of every (batch row b, head h): a state S of [dk, dv], fp32,
  *   forward :  S_t = g S_{t-1} + a_write k_t v_t^T,       o_t = a_read g S_{t-1}^T q_t + a_intra (q_t . k_t) v_t  (and so on within a chunk)
@@ -24,7 +24,7 @@ enum { PVDER_SEQ_MAX_HEAD = 128, PVDER_SEQ_MAX_SCANS = 3, PVDER_SEQ_MAX_WIDTH = 
 typedef struct pvder_seq_scan {
     const void *q, *k, *v;          /* [B, T, H, dk], [B, T, H, dk], [B, T, H, dv] */
     void *o;                        /* [B, T, H, dv]; rows at and behind lengths[b] are written as zeros */
-    int64_t q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h, o_b, o_t, o_h;
+    int64_t q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h, o_b, o_t, o_h;   /* q_t, k_t, v_t: 0 .. PVDER_SEQ_MAX_TOKEN_STRIDE bytes */
     const float *s_in;              /* state that comes in, NULL: zeros; element (i, j) of (b, h) at b s_b + h s_h + i s_k + j s_v */
     float *s_out;                   /* state that goes out, NULL: not wanted; same strides */
     int64_t s_b, s_h, s_k, s_v;

@@ -420,3 +420,6 @@ def test_a_long_cache_of_offsets(ops, gpu_device):
     assert torch.equal(ops.decay_attention(c["q"], c["k"], rows, c["log_decay"]), want)
     rows.copy_(c["q"])
     assert torch.equal(ops.decay_attention(rows, c["k"], c["v"], c["log_decay"]), want)
+    tokens = big.as_strided((1, 5, H, D), (0, 40_000_000, D, 1))       # tokens 80 MB apart
+    tokens.copy_(c["v"][:1, :5])
+    assert torch.equal(ops.decay_attention(c["q"][:1, :5], c["k"][:1, :5], tokens, c["log_decay"]), want[:1, :5])
