@@ -14,7 +14,6 @@ namespace {
 
 using namespace pvder_seq;
 
-constexpr int kSumBlocks = 512;            // blocks of the backward pass that leave partial sums: two for each CU
 
 // threads of a block: 256 where a wave holds whole rows, else one row's
 constexpr int block_of(int tpr) { return tpr > 64 ? tpr : 256; }
@@ -24,35 +23,55 @@ template <typename T, int NV> struct Row {
     float e[E];
 };
 
-// lane t of TPR holds the vectors t, t + TPR, ...
-template <typename T, int TPR, int NV> __device__ __forceinline__ void load(Row<T, NV> &r, const T *row, int t, int dim) {
+// lane t of TPR holds the vectors t, t + TPR, ...;  EVEN: the width is a multiple of a vector, which then is there whole or not at all
+template <typename T, bool EVEN> __device__ __forceinline__ typename Vec<T>::type load_vec(const T *row, int d, int D) {
+    if constexpr (EVEN) {
+        u4 u;
+        __builtin_memcpy(&u, row + (d < D ? d : 0), 16);
+        return __builtin_bit_cast(typename Vec<T>::type, d < D ? u : u4{0u, 0u, 0u, 0u});
+    } else {
+        return load_row<T>(row, d, D);
+    }
+}
+template <typename T, bool EVEN> __device__ __forceinline__ void store_vec(T *row, int d, int D, typename Vec<T>::type f) {
+    if constexpr (EVEN) {
+        if (d < D) __builtin_memcpy(row + d, &f, 16);
+    } else {
+        store_row<T>(row, d, D, f);
+    }
+}
+template <bool EVEN, typename T, int TPR, int NV> __device__ __forceinline__ void load(Row<T, NV> &r, const T *row, int t, int D) {
     constexpr int V = Vec<T>::N;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const typename Vec<T>::type f = load_row<T>(row, (i * TPR + t) * V, dim);
+        const typename Vec<T>::type f = load_vec<T, EVEN>(row, (i * TPR + t) * V, D);
 #pragma unroll
         for (int e = 0; e < V; ++e) r.e[i * V + e] = (float)f[e];
     }
 }
-template <typename T, int TPR, int NV> __device__ __forceinline__ void store(T *row, const Row<T, NV> &r, int t, int dim) {
+template <bool EVEN, typename T, int TPR, int NV> __device__ __forceinline__ void store(T *row, const Row<T, NV> &r, int t, int D) {
     constexpr int V = Vec<T>::N;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         typename Vec<T>::type f;
 #pragma unroll
         for (int e = 0; e < V; ++e) f[e] = (T)r.e[i * V + e];
-        store_row<T>(row, (i * TPR + t) * V, dim, f);
+        store_vec<T, EVEN>(row, (i * TPR + t) * V, D, f);
     }
 }
-// a parameter row of fp32: `zero` behind the width
-template <typename T, int TPR, int NV> __device__ __forceinline__ void load_param(Row<T, NV> &r, const float *p, int t, int dim, float otherwise) {
+// a row of fp32 weights: zeros behind the width, `otherwise` where there is none
+template <bool EVEN, typename T, int TPR, int NV> __device__ __forceinline__ void load_param(Row<T, NV> &r, const float *p, int t, int D, float otherwise) {
     constexpr int V = Vec<T>::N;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const int d = (i * TPR + t) * V + e;
-            r.e[i * V + e] = d < dim ? (p ? p[d] : otherwise) : 0.f;
+        for (int k = 0; k < V; k += 4) {
+            const int d = (i * TPR + t) * V + k;
+            f4 f;
+            if (p) f = load_vec<float, EVEN>(p, d, D);
+            else f = d < D ? f4{otherwise, otherwise, otherwise, otherwise} : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.e[i * V + k + e] = f[e];
         }
 }
 
@@ -71,109 +90,135 @@ template <int TPR> __device__ __forceinline__ float row_sum(float x, float *lds)
     return x;
 }
 
-// sigmoid(z) and 1 - sigmoid(z), both without cancellation
-__device__ __forceinline__ void sigmoids(float z, float &s, float &c) {
-    const float t = exp2f(-fabsf(z) * 1.44269504088896340736f), r = 1.f / (1.f + t);
+// sigmoid(z) and sigmoid(z) (1 - sigmoid(z)), without cancellation.  t is below 1, and zero where it would be no normal number.
+__device__ __forceinline__ void sigmoids(float z, float &s, float &sc) {
+    const float t = __builtin_amdgcn_exp2f(-fabsf(z) * 1.44269504088896340736f), r = __builtin_amdgcn_rcpf(1.f + t);
     s = z >= 0.f ? r : t * r;
-    c = z >= 0.f ? t * r : r;
-    if (z != z) s = c = z;
+    sc = t * r * r;
 }
 
-template <typename T, int TPR, int NV> __global__ __launch_bounds__(block_of(TPR)) void seq_norm_forward_kernel(const pvder_seq_norm a) {
+// Rows go round the blocks and the weights stay in registers: at a width of 2048 they are as many bytes as a row of all tensors.
+template <typename T, int TPR, int NV, bool EVEN> __global__ __launch_bounds__(block_of(TPR)) void seq_norm_forward_kernel(const pvder_seq_norm a) {
     constexpr int BLOCK = block_of(TPR), RPB = BLOCK / TPR, E = Row<T, NV>::E;
     __shared__ float lds[TPR > 64 ? TPR / 64 : 1];
-    const int t = threadIdx.x % TPR, D = a.width;
-    const long long r = blockIdx.x * (long long)RPB + threadIdx.x / TPR;
-    if (TPR <= 64 && r >= a.rows) return;
-    const bool on = r < a.rows;
-    const int dim = on ? D : 0;
-    Row<T, NV> y, h, z, w;
-    load<T, TPR, NV>(y, (const T *)a.y + r * a.y_r, t, dim);
-    load<T, TPR, NV>(h, (const T *)a.h + r * a.h_r, t, dim);
-    if (a.gate) load<T, TPR, NV>(z, (const T *)a.gate + r * a.gate_r, t, dim);
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = __builtin_fmaf(y.e[e], y.e[e], s);
-    const float ry = rsqrtf(row_sum<TPR>(s, lds) / (float)D + a.eps);
-    load_param<T, TPR, NV>(w, a.post, t, dim, 1.f);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        float u = y.e[e] * ry * w.e[e];
-        if (a.gate) { float sg, c; sigmoids(z.e[e], sg, c); u *= sg; }
-        y.e[e] = u;
-    }
-    load_param<T, TPR, NV>(w, a.scale, t, dim, 1.f);
-    s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        h.e[e] = __builtin_fmaf(w.e[e], y.e[e], h.e[e]);
-        s = __builtin_fmaf(h.e[e], h.e[e], s);
-    }
-    const float rh = rsqrtf(row_sum<TPR>(s, lds) / (float)D + a.eps);
-    store<T, TPR, NV>((T *)a.h_out + r * D, h, t, dim);
-    load_param<T, TPR, NV>(w, a.pre, t, dim, 1.f);
-#pragma unroll
-    for (int e = 0; e < E; ++e) h.e[e] *= rh * w.e[e];
-    store<T, TPR, NV>((T *)a.x_out + r * D, h, t, dim);
-    if (on && a.stats && t == 0) { a.stats[2 * r] = ry; a.stats[2 * r + 1] = rh; }
-}
-
-template <typename T, int TPR, int NV> __global__ __launch_bounds__(block_of(TPR)) void seq_norm_backward_kernel(const pvder_seq_norm a) {
-    constexpr int BLOCK = block_of(TPR), RPB = BLOCK / TPR, V = Vec<T>::N, E = Row<T, NV>::E;
-    __shared__ float lds[TPR > 64 ? TPR / 64 : 1];
-    __shared__ float sums[RPB > 1 ? BLOCK * E : 1];
     const int t = threadIdx.x % TPR, D = a.width, grp = threadIdx.x / TPR;
-    Row<T, NV> post, pre, scale, gpost, gpre, gscale;
-    load_param<T, TPR, NV>(post, a.post, t, D, 1.f);
-    load_param<T, TPR, NV>(pre, a.pre, t, D, 1.f);
-    load_param<T, TPR, NV>(scale, a.scale, t, D, 1.f);
-#pragma unroll
-    for (int e = 0; e < E; ++e) gpost.e[e] = gpre.e[e] = gscale.e[e] = 0.f;
     const float inv = 1.f / (float)D;
-    // (rows go round the blocks; every lane of a block takes as many turns: sums over more than a wave have a barrier in them)
+    Row<T, NV> post, pre, scale;
+    load_param<EVEN, T, TPR, NV>(post, a.post, t, D, 1.f);
+    load_param<EVEN, T, TPR, NV>(scale, a.scale, t, D, 1.f);
+    load_param<EVEN, T, TPR, NV>(pre, a.pre, t, D, 1.f);
+    // (every lane of a block takes as many turns: sums over more than a wave have a barrier in them)
     for (long long r0 = blockIdx.x * (long long)RPB; r0 < a.rows; r0 += gridDim.x * (long long)RPB) {
-        const long long r = r0 + grp;
-        const bool on = r < a.rows;
-        const int dim = on ? D : 0;
-        Row<T, NV> y, h, z, dh, dx;
-        load<T, TPR, NV>(y, (const T *)a.y + r * a.y_r, t, dim);
-        load<T, TPR, NV>(h, (const T *)a.h + r * a.h_r, t, dim);
-        load<T, TPR, NV>(z, (const T *)a.gate + r * a.gate_r, t, a.gate ? dim : 0);
-        load<T, TPR, NV>(dh, (const T *)a.dh + r * a.dh_r, t, a.dh ? dim : 0);
-        load<T, TPR, NV>(dx, (const T *)a.dx + r * a.dx_r, t, a.dx ? dim : 0);
-        const float ry = on ? a.stats[2 * r] : 0.f, rh = on ? a.stats[2 * r + 1] : 0.f;
+        const bool on = r0 + grp < a.rows;
+        const long long r = on ? r0 + grp : r0;
+        Row<T, NV> y, h, z;
+        load<EVEN, T, TPR, NV>(y, (const T *)a.y + r * a.y_r, t, D);
+        load<EVEN, T, TPR, NV>(h, (const T *)a.h + r * a.h_r, t, D);
+        if (a.gate) load<EVEN, T, TPR, NV>(z, (const T *)a.gate + r * a.gate_r, t, D);
         float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            float sg = 1.f, c = 0.f;
-            if (a.gate) sigmoids(z.e[e], sg, c);
-            const float u = y.e[e] * ry * post.e[e] * sg;
-            h.e[e] = __builtin_fmaf(scale.e[e], u, h.e[e]);
-            s = __builtin_fmaf(dx.e[e] * pre.e[e], h.e[e], s);
-        }
-        const float A = row_sum<TPR>(s, lds) * inv * rh * rh;
+        for (int e = 0; e < E; ++e) s = __builtin_fmaf(y.e[e], y.e[e], s);
+        const float ry = rsqrtf(row_sum<TPR>(s, lds) * inv + a.eps);
         s = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            float sg = 1.f, c = 0.f;
-            if (a.gate) sigmoids(z.e[e], sg, c);
-            const float n0 = y.e[e] * ry, n = n0 * post.e[e];
-            gpre.e[e] = __builtin_fmaf(dx.e[e] * h.e[e], rh, gpre.e[e]);
-            const float d = __builtin_fmaf(rh, dx.e[e] * pre.e[e] - h.e[e] * A, dh.e[e]);
-            const float du = d * scale.e[e];
-            gscale.e[e] = __builtin_fmaf(d, n * sg, gscale.e[e]);
-            gpost.e[e] = __builtin_fmaf(du * sg, n0, gpost.e[e]);
-            z.e[e] = du * n * sg * c;
-            dh.e[e] = d;
-            dx.e[e] = du * sg * post.e[e];
-            s = __builtin_fmaf(dx.e[e], y.e[e], s);
+            float u = y.e[e] * ry * post.e[e];
+            if (a.gate) { float sg, sc; sigmoids(z.e[e], sg, sc); u *= sg; }
+            h.e[e] = __builtin_fmaf(scale.e[e], u, h.e[e]);
+            s = __builtin_fmaf(h.e[e], h.e[e], s);
+        }
+        const float rh = rsqrtf(row_sum<TPR>(s, lds) * inv + a.eps);
+        if (!on) continue;                                 // (the block's last turn)
+        store<EVEN, T, TPR, NV>((T *)a.h_out + r * D, h, t, D);
+#pragma unroll
+        for (int e = 0; e < E; ++e) h.e[e] *= rh * pre.e[e];
+        store<EVEN, T, TPR, NV>((T *)a.x_out + r * D, h, t, D);
+        if (a.stats && t == 0) { a.stats[2 * r] = ry; a.stats[2 * r + 1] = rh; }
+    }
+}
+
+template <typename T, int TPR, int NV, bool EVEN> __global__ __launch_bounds__(block_of(TPR)) void seq_norm_backward_kernel(const pvder_seq_norm a) {
+    constexpr int BLOCK = block_of(TPR), RPB = BLOCK / TPR, V = Vec<T>::N, E = Row<T, NV>::E;
+    typedef typename Vec<T>::type vec;
+    // Rows of more than 4096 (16 elements a lane): h' and the sigmoid are taken a second time and the weights come from L2 row by row;
+    // held in registers they would not fit
+    constexpr bool LEAN = E > 8;
+    __shared__ float lds[TPR > 64 ? TPR / 64 : 1];
+    __shared__ float sums[RPB > 1 ? RPB * TPR * E : 1];
+    const int t = threadIdx.x % TPR, D = a.width, grp = threadIdx.x / TPR;
+    Row<T, NV> post, pre, scale, gpost, gpre, gscale;
+    auto weights = [&]() {
+        load_param<EVEN, T, TPR, NV>(post, a.post, t, D, 1.f);
+        load_param<EVEN, T, TPR, NV>(pre, a.pre, t, D, 1.f);
+        load_param<EVEN, T, TPR, NV>(scale, a.scale, t, D, 1.f);
+    };
+    if constexpr (!LEAN) weights();
+#pragma unroll
+    for (int e = 0; e < E; ++e) gpost.e[e] = gpre.e[e] = gscale.e[e] = 0.f;
+    const float inv = 1.f / (float)D;
+    for (long long r0 = blockIdx.x * (long long)RPB; r0 < a.rows; r0 += gridDim.x * (long long)RPB) {
+        const bool on = r0 + grp < a.rows;
+        const long long r = on ? r0 + grp : r0;
+        vec y[NV], h[NV], z[NV], dh[NV], dx[NV];
+        auto row = [&](vec *f, const void *p, int64_t stride) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (p) f[i] = load_vec<T, EVEN>((const T *)p + r * stride, (i * TPR + t) * V, D);
+                else f[i] = __builtin_bit_cast(vec, u4{0u, 0u, 0u, 0u});
+            }
+        };
+        row(y, a.y, a.y_r);
+        row(h, a.h, a.h_r);
+        row(z, a.gate, a.gate_r);
+        row(dx, a.dx, a.dx_r);
+        row(dh, a.dh, a.dh_r);
+        const float ry = a.stats[2 * r], rh = a.stats[2 * r + 1];
+        if constexpr (LEAN) weights();
+        Row<T, NV> hn, sg, sc, dn;
+        auto branch = [&](int e) {                          // element e of h', the sigmoid and its derivative
+            const int i = e / V, k = e % V;
+            sg.e[e] = 1.f;
+            sc.e[e] = 0.f;
+            if (a.gate) sigmoids((float)z[i][k], sg.e[e], sc.e[e]);
+            hn.e[e] = __builtin_fmaf(scale.e[e], (float)y[i][k] * ry * post.e[e] * sg.e[e], (float)h[i][k]);
+        };
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            branch(e);
+            s = __builtin_fmaf((float)dx[e / V][e % V] * pre.e[e], hn.e[e], s);
+        }
+        const float A = row_sum<TPR>(s, lds) * inv * rh * rh;
+        if constexpr (LEAN) weights();
+        s = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int i = e / V, k = e % V;
+            if constexpr (LEAN) branch(e);
+            const float x = (float)dx[i][k], n0 = (float)y[i][k] * ry, n = n0 * post.e[e];
+            const float d = __builtin_fmaf(rh, x * pre.e[e] - hn.e[e] * A, (float)dh[i][k]), du = d * scale.e[e];
+            if (on) {                                      // (a row past the end stands in for the block's first)
+                gpre.e[e] = __builtin_fmaf(x * hn.e[e], rh, gpre.e[e]);
+                gscale.e[e] = __builtin_fmaf(d, n * sg.e[e], gscale.e[e]);
+                gpost.e[e] = __builtin_fmaf(du * sg.e[e], n0, gpost.e[e]);
+            }
+            z[i][k] = (T)(sc.e[e] * du * n);
+            dh[i][k] = (T)d;
+            dn.e[e] = du * sg.e[e] * post.e[e];
+            s = __builtin_fmaf(dn.e[e], (float)y[i][k], s);
         }
         const float B = row_sum<TPR>(s, lds) * inv * ry * ry;
+        if (!on) continue;
 #pragma unroll
-        for (int e = 0; e < E; ++e) dx.e[e] = ry * (dx.e[e] - y.e[e] * B);
-        store<T, TPR, NV>((T *)a.dh_out + r * D, dh, t, dim);
-        store<T, TPR, NV>((T *)a.dy_out + r * D, dx, t, dim);
-        if (a.gate) store<T, TPR, NV>((T *)a.dgate_out + r * D, z, t, dim);
+        for (int i = 0; i < NV; ++i) {
+            const int d0 = (i * TPR + t) * V;
+            vec f;
+#pragma unroll
+            for (int k = 0; k < V; ++k) f[k] = (T)(ry * (dn.e[i * V + k] - (float)y[i][k] * B));
+            store_vec<T, EVEN>((T *)a.dh_out + r * D, d0, D, dh[i]);
+            store_vec<T, EVEN>((T *)a.dy_out + r * D, d0, D, f);
+            if (a.gate) store_vec<T, EVEN>((T *)a.dgate_out + r * D, d0, D, z[i]);
+        }
     }
     if (!a.dparam) return;
     float *out = (gridDim.x > 1 ? a.workspace : a.dparam) + blockIdx.x * 3ll * D;
@@ -183,15 +228,16 @@ template <typename T, int TPR, int NV> __global__ __launch_bounds__(block_of(TPR
         if constexpr (RPB > 1) {
             __syncthreads();
 #pragma unroll
-            for (int e = 0; e < E; ++e) sums[e * BLOCK + threadIdx.x] = v.e[e];
-            __syncthreads();
-            if (grp == 0)
+            for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-#pragma unroll 1
-                    for (int g = 1; g < RPB; ++g) v.e[e] += sums[e * BLOCK + g * TPR + t];
-        }
-        if (grp == 0)
+                for (int e = 0; e < V; ++e) sums[grp * (TPR * E) + (i * TPR + t) * V + e] = v.e[i * V + e];
+            __syncthreads();
+            for (int d = threadIdx.x; d < D; d += BLOCK) {
+                float x = sums[d];
+                for (int g = 1; g < RPB; ++g) x += sums[g * (TPR * E) + d];
+                out[k * D + d] = x;
+            }
+        } else {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -199,6 +245,7 @@ template <typename T, int TPR, int NV> __global__ __launch_bounds__(block_of(TPR
                     const int d = (i * TPR + t) * V + e;
                     if (d < D) out[k * D + d] = v.e[i * V + e];
                 }
+        }
     }
 }
 
@@ -219,38 +266,43 @@ __global__ __launch_bounds__(256) void seq_norm_sum_kernel(const float *__restri
     }
 }
 
-struct Shape { int tpr, nv; };
-// lanes to a row and vectors to a lane: the fewest lanes that hold the row at up to 16 elements a lane, 4 lanes at least
-Shape shape_of(int width, int dtype) {
-    const int v = dtype == PVDER_SEQ_BF16 ? 8 : 4, nv = 16 / v;
+// lanes to a row: the fewest that hold it at 8 elements a lane, 4 at least; 512 lanes hold 16 where they have to
+int lanes_of(int width) {
     int tpr = 4;
-    while (tpr * v * nv < width) tpr <<= 1;
-    return {tpr, nv};
+    while (tpr * 8 < width && tpr < 512) tpr <<= 1;
+    return tpr;
 }
 int rows_per_block(int tpr) { return block_of(tpr) / tpr; }
-long long sum_blocks(const pvder_seq_norm *a, int tpr) {
-    const long long need = (a->rows + rows_per_block(tpr) - 1) / rows_per_block(tpr);
-    return need < kSumBlocks ? need : kSumBlocks;
+// blocks for `rows` rows, `waves` of them on each of the 256 CUs at most, all with as many turns
+long long blocks_of(long long rows, int tpr, int waves) {
+    const long long need = (rows + rows_per_block(tpr) - 1) / rows_per_block(tpr), most = 256ll * waves * 64 / block_of(tpr);
+    const long long turns = (need + most - 1) / most;
+    return (need + turns - 1) / turns;
 }
+constexpr int kForwardWaves = 24, kBackwardWaves = 12;
 
-template <typename T, int TPR> int run(const pvder_seq_norm &a, bool back, hipStream_t st) {
-    constexpr int NV = 16 / Vec<T>::N, BLOCK = block_of(TPR), RPB = BLOCK / TPR;
+template <typename T, int TPR, int NV, bool EVEN> void start(const pvder_seq_norm &a, bool back, hipStream_t st) {
+    constexpr int BLOCK = block_of(TPR);
+    const unsigned blocks = (unsigned)blocks_of(a.rows, TPR, back ? kBackwardWaves : kForwardWaves);
     if (back) {
-        const long long blocks = sum_blocks(&a, TPR);
-        seq_norm_backward_kernel<T, TPR, NV><<<dim3((unsigned)blocks), dim3(BLOCK), 0, st>>>(a);
+        seq_norm_backward_kernel<T, TPR, NV, EVEN><<<dim3(blocks), dim3(BLOCK), 0, st>>>(a);
         if (a.dparam && blocks > 1)
             seq_norm_sum_kernel<<<dim3((3 * a.width + 31) / 32), dim3(256), 0, st>>>(a.workspace, a.dparam, (int)blocks, 3 * a.width);
     } else {
-        const long long blocks = (a.rows + RPB - 1) / RPB;
-        if (blocks > 0x7fffffffll) return kEinval;
-        seq_norm_forward_kernel<T, TPR, NV><<<dim3((unsigned)blocks), dim3(BLOCK), 0, st>>>(a);
+        seq_norm_forward_kernel<T, TPR, NV, EVEN><<<dim3(blocks), dim3(BLOCK), 0, st>>>(a);
     }
+}
+
+template <typename T, int TPR, int PER_LANE = 8> int run(const pvder_seq_norm &a, bool back, hipStream_t st) {
+    constexpr int NV = PER_LANE / Vec<T>::N;
+    if (a.width % Vec<T>::N == 0) start<T, TPR, NV, true>(a, back, st);
+    else start<T, TPR, NV, false>(a, back, st);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : -(int)e;
 }
 
 template <typename T> int pick(const pvder_seq_norm &a, bool back, hipStream_t st) {
-    switch (shape_of(a.width, a.dtype).tpr) {
+    switch (lanes_of(a.width)) {
         case 4: return run<T, 4>(a, back, st);
         case 8: return run<T, 8>(a, back, st);
         case 16: return run<T, 16>(a, back, st);
@@ -258,7 +310,7 @@ template <typename T> int pick(const pvder_seq_norm &a, bool back, hipStream_t s
         case 64: return run<T, 64>(a, back, st);
         case 128: return run<T, 128>(a, back, st);
         case 256: return run<T, 256>(a, back, st);
-        default: return run<T, 512>(a, back, st);
+        default: return a.width <= 4096 ? run<T, 512>(a, back, st) : run<T, 512, 16>(a, back, st);
     }
 }
 
@@ -272,7 +324,7 @@ bool ok(const pvder_seq_norm *a) {
 extern "C" int64_t pvder_seq_norm_workspace(const pvder_seq_norm *a) {
     if (!ok(a)) return kEinval;
     if (!a->dparam || a->rows == 0) return 0;
-    const long long blocks = sum_blocks(a, shape_of(a->width, a->dtype).tpr);
+    const long long blocks = blocks_of(a->rows, lanes_of(a->width), kBackwardWaves);
     return blocks > 1 ? blocks * 3 * a->width : 0;
 }
 
