@@ -20,6 +20,7 @@ LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libpvder_hip.so")
 SEQUENCE_CSRC = os.path.join(CSRC, "sequence")
 SEQUENCE_LIB_PATH = os.path.join(LIB_DIR, "libpvder_sequence.so")
+SEQUENCE_TORCH_PATH = os.path.join(LIB_DIR, "_pvder_sequence_torch.so")
 
 EINVAL = -10001
 ETIMEOUT = -10003             # include/pvder_hip.h PVDER_ETIMEOUT: the device never wrote the host mirror's sequence word
@@ -103,13 +104,14 @@ def hipcc_path() -> str:
     return shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 
 
-def _build(lib_path: str, srcs, deps, flags, force: bool, verbose: bool) -> str:
+def _build(lib_path: str, deps, cmd, force: bool, verbose: bool) -> str:
+    """Run ``cmd`` + the output's name unless ``lib_path`` is newer than everything it is made of."""
     if (not force and os.path.exists(lib_path)
             and all(os.path.getmtime(d) <= os.path.getmtime(lib_path) for d in deps)):
         return lib_path
     os.makedirs(LIB_DIR, exist_ok=True)
     tmp = "%s.%d.tmp" % (lib_path, os.getpid())          # build aside, then rename: never a half-written library
-    cmd = [hipcc_path()] + flags + ["-fPIC", "-shared", "-I" + INCLUDE, "-I" + CSRC, "-o", tmp] + srcs
+    cmd = cmd + ["-o", tmp]
     if verbose:
         print(" ".join(cmd))
     try:
@@ -126,17 +128,37 @@ def build_native(force: bool = False, verbose: bool = False) -> str:
     srcs = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(".hip")]
     deps = srcs + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hpp")]
     deps += [os.path.join(INCLUDE, "pvder_hip.h"), os.path.join(INCLUDE, "pvder_agent.h")]
-    _build(LIB_PATH, srcs, deps, HIPCC_FLAGS, force, verbose)
+    _build(LIB_PATH, deps, [hipcc_path()] + HIPCC_FLAGS + ["-fPIC", "-shared", "-I" + INCLUDE, "-I" + CSRC] + srcs, force, verbose)
     build_sequence(force, verbose)
     return LIB_PATH
 
 
 def build_sequence(force: bool = False, verbose: bool = False) -> str:
-    """Compile csrc/sequence/*.hip for gfx950 into gym_PVDER_amd/lib/libpvder_sequence.so (in-tree)."""
+    """Compile csrc/sequence/*.hip for gfx950 into gym_PVDER_amd/lib/libpvder_sequence.so (in-tree), and the torch binding that
+    calls it, csrc/sequence/torch_binding.cpp, with the host compiler."""
     names = sorted(os.listdir(SEQUENCE_CSRC))
     srcs = [os.path.join(SEQUENCE_CSRC, f) for f in names if f.endswith(".hip")]
-    deps = [os.path.join(SEQUENCE_CSRC, f) for f in names] + [os.path.join(INCLUDE, "pvder_sequence.h")]
-    return _build(SEQUENCE_LIB_PATH, srcs, deps, SEQUENCE_HIPCC_FLAGS, force, verbose)
+    header = os.path.join(INCLUDE, "pvder_sequence.h")
+    deps = srcs + [os.path.join(SEQUENCE_CSRC, f) for f in names if f.endswith(".hpp")] + [header]
+    _build(SEQUENCE_LIB_PATH, deps, [hipcc_path()] + SEQUENCE_HIPCC_FLAGS + ["-fPIC", "-shared", "-I" + INCLUDE] + srcs, force, verbose)
+    binding = os.path.join(SEQUENCE_CSRC, "torch_binding.cpp")
+    if (not force and os.path.exists(SEQUENCE_TORCH_PATH)
+            and all(os.path.getmtime(d) <= os.path.getmtime(SEQUENCE_TORCH_PATH) for d in (binding, header))):
+        return SEQUENCE_LIB_PATH                         # (without importing torch)
+    import sysconfig
+    import torch
+    inc = os.path.join(os.path.dirname(torch.__file__), "include")
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_pvder_sequence_torch",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+           "-I" + INCLUDE, "-isystem" + inc, "-isystem" + os.path.join(inc, "torch", "csrc", "api", "include"),
+           "-isystem" + os.path.join(rocm, "include"), "-isystem" + sysconfig.get_paths()["include"], binding,
+           "-L" + LIB_DIR, "-l:libpvder_sequence.so", "-Wl,-rpath,$ORIGIN", "-L" + libs, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip",
+           "-ltorch", "-ltorch_python"]
+    _build(SEQUENCE_TORCH_PATH, [binding, header], cmd, force, verbose)
+    return SEQUENCE_LIB_PATH
 
 
 _lib = None
@@ -266,7 +288,7 @@ def sequence_lib() -> C.CDLL:
     missing = [s for s in SEQUENCE_SYMBOLS if not hasattr(L, s)]
     if missing:
         raise ImportError("libpvder_sequence.so lacks symbols: %s" % missing)
-    # the arguments are the structs of include/pvder_sequence.h as bytes (agents/sequence_ops.py packs them)
+    # the arguments are the structs of include/pvder_sequence.h
     for name in ("pvder_seq_attn_run", "pvder_seq_step_run", "pvder_seq_norm_forward", "pvder_seq_norm_backward"):
         f = getattr(L, name)
         f.restype = C.c_int
@@ -277,3 +299,24 @@ def sequence_lib() -> C.CDLL:
         f.argtypes = [C.c_void_p]
     _sequence_lib = L
     return L
+
+
+_sequence_torch = None
+
+
+def sequence_torch():
+    """The torch binding of the sequence operators (csrc/sequence/torch_binding.cpp).  Raises if it or its library is missing."""
+    global _sequence_torch
+    if _sequence_torch is None:
+        sequence_lib()
+        if not os.path.exists(SEQUENCE_TORCH_PATH):
+            raise ImportError("%s not found -- run `python -c 'import __graft_entry__ as g; g.build()'`" % SEQUENCE_TORCH_PATH)
+        import importlib.machinery
+        import importlib.util
+        name = "_pvder_sequence_torch"
+        loader = importlib.machinery.ExtensionFileLoader(name, SEQUENCE_TORCH_PATH)
+        spec = importlib.util.spec_from_file_location(name, SEQUENCE_TORCH_PATH, loader=loader)
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+        _sequence_torch = module
+    return _sequence_torch

@@ -281,7 +281,7 @@ def _norm_run(ops, c, eps=1e-6, which=("dh", "dx")):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("gate,scale", [(True, True), (False, False), (True, False)])
+@pytest.mark.parametrize("gate,scale", [(True, True), (False, False), (True, False), (False, True)])
 @pytest.mark.parametrize("R,D", [(1, 1), (1, 128), (3, 3), (5, 16), (300, 17), (1025, 100), (64, 128), (7, 513), (33, 1024), (2100, 64), (10, 2048),
                                  (3, 4100), (5, 8192), (2, 8191)])
 def test_norm(ops, gpu_device, R, D, gate, scale, dtype):
@@ -320,6 +320,28 @@ def test_norm_layouts_and_parts(ops, gpu_device, dtype):
     e = {n: x[:0] if n in ("h", "y", "gate", "dh", "dx") else x for n, x in c.items()}
     got = _norm_run(ops, e)
     assert got["h"].shape == (0, 48) and not got["dpost"].any() and got["dgate"].shape == (0, 48)
+
+
+def test_each_gradient_by_itself(ops, gpu_device):
+    """Any one tensor may be the only one that asks for a gradient."""
+    for gate, scale in ((True, True), (False, True), (True, False)):
+        c = _norm_case(30, 40, torch.float32, gpu_device, gate, scale)
+        whole = _norm_run(ops, c)
+        for n in ("h", "y", "gate", "post", "pre", "scale"):
+            if c[n] is not None:
+                d = dict(c, **{n: c[n].detach().requires_grad_()})
+                h, x = ops.gated_residual_norm(d["h"], d["y"], d["post"], d["pre"], gate=d["gate"], scale=d["scale"])
+                assert torch.equal(torch.autograd.grad([h, x], [d[n]], [c["dh"], c["dx"]])[0], whole["d" + n]), n
+    for state in (True, False):
+        c = _case(2, 40, 2, 16, 24, torch.float32, gpu_device, True, state)
+        whole = _run(ops, c)
+        for n in ("q", "k", "v", "s0"):
+            if c[n] is not None:
+                d = dict(c, **{n: c[n].detach().requires_grad_()})
+                r = ops.decay_attention(d["q"], d["k"], d["v"], d["log_decay"], initial_state=d["s0"], starts=d["starts"], lengths=d["lengths"],
+                                        output_final_state=state)
+                got, = torch.autograd.grad(r, [d[n]], [c["do"], c["ds"]] if state else [c["do"]])
+                assert torch.equal(got, whole["d" + n]), n
 
 
 def test_norm_differences(ops, gpu_device):
@@ -423,3 +445,29 @@ def test_a_long_cache_of_offsets(ops, gpu_device):
     tokens = big.as_strided((1, 5, H, D), (0, 40_000_000, D, 1))       # tokens 80 MB apart
     tokens.copy_(c["v"][:1, :5])
     assert torch.equal(ops.decay_attention(c["q"][:1, :5], c["k"][:1, :5], tokens, c["log_decay"]), want[:1, :5])
+
+
+def test_a_second_derivative_is_refused(ops, gpu_device):
+    c, nc = _case(1, 9, 1, 8, 8, torch.float32, gpu_device), _norm_case(4, 8, torch.float32, gpu_device)
+    q = c["q"].detach().requires_grad_()
+    out = ops.decay_attention(q, c["k"], c["v"], c["log_decay"])
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad([out], [q], [c["do"]], create_graph=True)
+    y = nc["y"].detach().requires_grad_()
+    h, _ = ops.gated_residual_norm(nc["h"], y, nc["post"], nc["pre"])
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad([h], [y], [nc["dh"]], create_graph=True)
+
+
+def test_inputs_changed_before_the_backward_pass_are_noticed(ops, gpu_device):
+    c = _case(1, 9, 1, 8, 8, torch.float32, gpu_device)
+    q, k = c["q"].detach().clone().requires_grad_(), c["k"].clone()
+    out = ops.decay_attention(q, k, c["v"], c["log_decay"])
+    k.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    state = torch.zeros(1, 1, 8, 8, device=gpu_device)
+    loss = (state * torch.ones(1, device=gpu_device, requires_grad=True)).sum()
+    ops.decay_attention_step(c["q"][:, 0], c["k"][:, 0], c["v"][:, 0], c["log_decay"], state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
