@@ -24,12 +24,33 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// The parts of a chunk's work are scheduled by themselves: mixed, their operands do not fit the registers
+__device__ __forceinline__ void phase() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The value as it is at this place: keeps what a rare branch computes from it out of the registers of the whole loop
+__device__ __forceinline__ int here(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // ---- the two element types: an operand fragment is 16 bytes per lane, VPL contraction slots, KW of them over the wave ----
 template <typename T> struct Ty;
 
 template <> struct Ty<__bf16> {
     typedef b8 frag;
-    static constexpr int VPL = 8, KW = 32, TT = 2, PAD = 8, PARTS = 3;
+    static constexpr int VPL = 8, KW = 32, TT = 2;
+    // LDS tiles, rows of W elements in pieces of 16 bytes.  Tiles that are read by columns (4 rows of 64 bytes together) have rows 64
+    // bytes apart in the 256 bytes of the banks, those that are read by rows (a piece of 8 rows together) 16.  All places of a lane are
+    // one register and constants.
+    static constexpr int row(int w) { return w == 32 ? 32 : w + 32; }
+    static constexpr int size(int w) { return KW * row(w); }
+    // (128 wide they are turned instead: with the 16 bytes eight waves of a CU would not find room in its LDS)
+    static constexpr int size_rows(int w) { return KW * (w == 128 ? w : w + 8); }
+    template <int W> static __device__ __forceinline__ int at(int r, int piece) { return r * row(W) + 8 * piece; }
+    template <int W> static __device__ __forceinline__ int at_rows(int r, int piece) { return W == 128 ? r * W + 8 * (piece ^ (r & 7)) : r * (W + 8) + 8 * piece; }
     // accumulator row mm (0..15) of tile t within a group of KW rows
     static __device__ __forceinline__ int tile_row(int t, int mm) { return 8 * (mm >> 2) + 4 * t + (mm & 3); }
     static __device__ __forceinline__ f4 mfma(frag a, frag b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -38,24 +59,24 @@ template <> struct Ty<__bf16> {
         const f8 x = {t[0].x, t[0].y, t[0].z, t[0].w, t[1].x, t[1].y, t[1].z, t[1].w};
         return __builtin_convertvector(x, b8);
     }
-    // w_y v_y as PARTS summands of 8 bits each: the state is an fp32 sum of fp32 products, as it would be without matrix cores
-    // (one rounding to bf16 would be 2^-9 of every term and shows in the state that goes out)
-    static __device__ __forceinline__ void weighted(frag v, const float *w, frag *part) {
+    // w_y v_y as P summands of 8 bits each, P - 1 of them below the first: three are fp32's 24 bits, so a state that is returned is an fp32
+    // sum of fp32 products; two (2^-17 of each term) where only outputs of 8 bits are made of it.  One (2^-9) would show there too.
+    template <int P> static __device__ __forceinline__ void weighted(frag v, const float *w, frag *part) {
         f8 x = __builtin_convertvector(v, f8);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] *= w[e];
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
+        for (int p = 0; p < P; ++p) {
             part[p] = __builtin_convertvector(x, b8);
-            if (p + 1 < PARTS) x -= __builtin_convertvector(part[p], f8);
+            if (p + 1 < P) x -= __builtin_convertvector(part[p], f8);
         }
     }
-    // column fragment of an LDS tile [KW][W]: slots = rows VPL g + e, this lane's column = group base + tile_row(t, m)
-    template <int W> static __device__ __forceinline__ frag column(const __bf16 *tile, int col0, int t, int m, int g) {
-        const __bf16 *p = tile + (size_t)(8 * g + (m >> 2)) * (W + PAD) + col0 + 8 * (m & 3) + 4 * t;
+    // column fragment of an LDS tile [KW][W]: slots = rows VPL g + e, this lane's column = 32 (j / 2) + tile_row(j % 2, m)
+    template <int W> static __device__ __forceinline__ frag column(const __bf16 *tile, int j, int m, int g) {
+        const __bf16 *p = tile + at<W>(8 * g + (m >> 2), 4 * (j >> 1) + (m & 3)) + 4 * (j & 1);
         typedef __attribute__((address_space(3))) s4 lds4;
         const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)p);
-        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + 4 * (W + PAD)));
+        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4 *)(p + 4 * row(W)));
         typedef short s8 __attribute__((ext_vector_type(8)));
         const s8 r = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
         return __builtin_bit_cast(b8, r);
@@ -64,7 +85,11 @@ template <> struct Ty<__bf16> {
 
 template <> struct Ty<float> {
     typedef f4 frag;
-    static constexpr int VPL = 4, KW = 16, TT = 1, PAD = 4, PARTS = 1;
+    static constexpr int VPL = 4, KW = 16, TT = 1;
+    static constexpr int size(int w) { return KW * (w + 4); }
+    static constexpr int size_rows(int w) { return KW * (w + 4); }
+    template <int W> static __device__ __forceinline__ int at(int row, int piece) { return row * (W + 4) + 4 * piece; }
+    template <int W> static __device__ __forceinline__ int at_rows(int row, int piece) { return row * (W + 4) + 4 * piece; }
     static __device__ __forceinline__ int tile_row(int, int mm) { return mm; }
     static __device__ __forceinline__ f4 mfma(frag a, frag b, f4 c) {
 #pragma unroll
@@ -72,56 +97,62 @@ template <> struct Ty<float> {
         return c;
     }
     static __device__ __forceinline__ frag operand(const f4 *t) { return t[0]; }
-    static __device__ __forceinline__ void weighted(frag v, const float *w, frag *part) {
+    template <int> static __device__ __forceinline__ void weighted(frag v, const float *w, frag *part) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) part[0][e] = v[e] * w[e];
     }
-    template <int W> static __device__ __forceinline__ frag column(const float *tile, int col0, int, int m, int g) {
-        const float *p = tile + (size_t)(4 * g) * (W + PAD) + col0 + m;
-        return frag{p[0], p[W + PAD], p[2 * (W + PAD)], p[3 * (W + PAD)]};
+    template <int W> static __device__ __forceinline__ frag column(const float *tile, int j, int m, int g) {
+        const float *p = tile + 4 * g * (W + 4) + 16 * j + m;
+        return frag{p[0], p[W + 4], p[2 * (W + 4)], p[3 * (W + 4)]};
     }
 };
 
+// LDS of a wave: a chunk's rows of Q, K and V
+template <typename T> constexpr int tile_bytes(int dkp, int dvs) { return (Ty<T>::size(dkp) + Ty<T>::size(dvs) + Ty<T>::size_rows(dkp > dvs ? dkp : dvs)) * (int)sizeof(T); }
+
 struct Args {
     pvder_seq_attn a;
-    int seg_len, n_sib;                     // tokens of a piece; waves of one (b, h, piece): all strips of all scans
-    int sib0[PVDER_SEQ_MAX_SCANS + 1];      // first wave of each scan
-    long long n_groups, per_sib;            // (b, h, piece) triples; workspace floats of one wave's state
-    float *carry;                           // [scan][b][h][piece]: what a piece leaves of the state before it, < 0: nothing (a start)
+    int seg_len, n_sib;                     // tokens of a piece; strips of one (b, h, piece), all scans together
+    int sib0[PVDER_SEQ_MAX_SCANS + 1];      // first strip of each scan
+    unsigned n_groups;                      // (b, h, piece) triples
+    long long per_sib;            // workspace floats of one strip's state
+    float *carry;                           // [scan][b][h][piece]: what a piece leaves of the state before it (0 behind a start)
 };
 
-// Which (b, h, piece) and which wave of it a block is.  Blocks are dealt to the eight XCDs in turn: the waves of one triple read
+// Which (b, h, piece) and which of its scans a block is.  Blocks are dealt to the eight XCDs in turn: the scans of one triple read
 // the same tensors, so they get block numbers that are 8 apart and share one L2.
-__device__ __forceinline__ bool whose(const Args &A, long long &grp, int &sib) {
-    const long long id = blockIdx.x, row = id / (8 * A.n_sib);
-    const int in = (int)(id - row * 8 * A.n_sib);
-    sib = in >> 3;
-    grp = row * 8 + (in & 7);
+__device__ __forceinline__ bool whose(const Args &A, unsigned &grp, int &sc) {
+    const unsigned row = (blockIdx.x >> 3) / (unsigned)A.n_sib;
+    sc = (int)((blockIdx.x >> 3) - row * (unsigned)A.n_sib);
+    grp = row * 8 + (blockIdx.x & 7);
     return grp < A.n_groups;
 }
 
-// WHOLE: heads of exactly DKP and a multiple of DVS
-template <typename T, int DKP, int DVS, bool WHOLE, bool STATE_ONLY>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(DKP * DVS > 4096 ? 1 : 2)))
+// A block is one wave: one strip of one scan over one (b, h, piece).  Strips of a head in one block, on one CU, were up to twice as slow
+// (128 x 128, 160 tokens: 23 us against 12): four waves that walk in step ask the CU's L1 and LDS for the same at the same time.
+// WHOLE: heads of exactly DKP and a multiple of DVS.  STATE_ONLY: only the state behind a piece is wanted.  PARTS: see `weighted`.
+template <typename T, int DKP, int DVS, bool WHOLE, bool STATE_ONLY, int PARTS>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(2)))
 void seq_scan_kernel(const Args A) {
     typedef Ty<T> Y;
     typedef typename Y::frag frag;
     constexpr int C = Y::KW, NT = C / 16, TT = Y::TT, V = Y::VPL;
     constexpr int KS = DKP / Y::KW, VS = DVS / Y::KW, NI = DKP / 16, NJ = DVS / 16;
-    __shared__ __attribute__((aligned(16))) T ldsK[C * (DKP + Y::PAD)], ldsV[C * (DVS + Y::PAD)];
+    extern __shared__ __attribute__((aligned(16))) char lds[];
 
-    long long grp;
-    int sib;
-    if (!whose(A, grp, sib)) return;
-    int sc = 0;
+    unsigned grp;
+    int sc;
+    if (!whose(A, grp, sc)) return;
+    const int sib = sc;
+    sc = 0;
     while (sc + 1 < A.a.n_scans && sib >= A.sib0[sc + 1]) ++sc;
     const pvder_seq_scan &S = A.a.scan[sc];
     const int strip = sib - A.sib0[sc], dv0 = strip * DVS;
+    T *ldsK = (T *)lds, *ldsV = ldsK + Y::size(DKP), *ldsQ = ldsV + Y::size(DVS);       // (ldsQ takes the output when Q has been read)
     const int nseg = A.a.segments;
-    const int seg = (int)(grp % nseg);
-    const long long bh = grp / nseg;
-    const int h = (int)(bh % A.a.H), b = (int)(bh / A.a.H);
-    const int lane = threadIdx.x, g = lane >> 4, m = lane & 15;
+    const unsigned bh = nseg == 1 ? grp : grp / (unsigned)nseg;
+    const int seg = (int)(grp - bh * (unsigned)nseg), b = (int)(bh / (unsigned)A.a.H), h = (int)(bh - (unsigned)b * (unsigned)A.a.H);
+    const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
     const bool rev = S.reverse != 0;
     const int DK = S.dk, DV = S.dv - dv0;                 // columns of this strip's rows that exist: dv0 .. dv0 + DV
 
@@ -144,24 +175,31 @@ void seq_scan_kernel(const Args A) {
 
     // ---- the state that comes in: element (i, j, r) is S[KW (i / TT) + tile_row(i % TT, 4 g + r)][KW (j / TT) + tile_row(j % TT, m)]
     f4 s[NI][NJ];
-    const bool first = rev ? seg == nseg - 1 : seg == 0;
-    float *ws = A.a.workspace ? A.a.workspace + ((grp * A.n_sib + sib) * A.per_sib) + lane * 4 : nullptr;
-    if (!STATE_ONLY && nseg > 1) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) s[i][j] = *(const f4 *)(ws + (i * NJ + j) * 256);
-    } else if (!STATE_ONLY && first && S.s_in) {
-        const float *p = S.s_in + b * S.s_b + h * S.s_h;
+    auto state_elements = [&](auto &&f) {                   // f(i, j, r, whether the head has the element, its offset in bytes)
+        const int g4 = 4 * (here(lane) >> 4), mm = here(lane) & 15;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int dk = Y::KW * (i / TT) + Y::tile_row(i % TT, 4 * g + r), dv = Y::KW * (j / TT) + Y::tile_row(j % TT, m);
-                    s[i][j][r] = dk < DK && dv < DV ? p[dk * S.s_k + (dv0 + dv) * S.s_v] : 0.f;
+                    const int dk = Y::KW * (i / TT) + Y::tile_row(i % TT, g4 + r), dv = Y::KW * (j / TT) + Y::tile_row(j % TT, mm);
+                    f(i, j, r, dk < DK && dv < DV, (unsigned)dk * (unsigned)(4 * S.s_k) + (unsigned)(dv0 + dv) * (unsigned)(4 * S.s_v));
                 }
+    };
+    const bool first = rev ? seg == nseg - 1 : seg == 0;
+    float *ws = A.a.workspace ? A.a.workspace + (((long long)grp * A.n_sib + sib) * A.per_sib) + lane * 4 : nullptr;
+    if (!STATE_ONLY && nseg > 1) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) s[i][j] = *(const f4 *)(ws + (i * NJ + j) * 256);
+    } else if (!STATE_ONLY && first && S.s_in) {
+        const gbytes p = shared_base(S.s_in + b * S.s_b + h * S.s_h);
+        state_elements([&](int i, int j, int r, bool is, unsigned at) {
+            const float x = *(const __attribute__((address_space(1))) float *)(p + (is ? at : 0u));
+            s[i][j][r] = is ? x : 0.f;
+        });
     } else {
 #pragma unroll
         for (int i = 0; i < NI; ++i)
@@ -178,247 +216,301 @@ void seq_scan_kernel(const Args A) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int x = 16 * nt + m, y = V * g + 4 * t + r, d = rev ? y - x : x - y;
-                dw[nt][t][r] = d >= 0 ? S.a_intra * power(lg, d) : 0.f;
+                const float w = S.a_intra * power(lg, d);
+                dw[nt][t][r] = d >= 0 ? w : 0.f;
             }
     int n_have = 0;
     auto by_length = [&](int n) {
         if (n == n_have) return;
         n_have = n;
+        const int g = here(lane) >> 4, m = here(lane) & 15;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             const int y = V * g + e, d = rev ? y + 1 : n - 1 - y;
-            wy[e] = y < n ? S.a_write * power(lg, d) : 0.f;
+            const float w = S.a_write * power(lg, d);
+            wy[e] = y < n ? w : 0.f;
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int x = 16 * nt + m, d = rev ? n - 1 - x : x + 1;
-            rx[nt] = x < n ? S.a_read * power(lg, d) : 0.f;
+            const float w = S.a_read * power(lg, d);
+            rx[nt] = x < n ? w : 0.f;
         }
         gn = power(lg, n);
     };
 
-    // ---- loads of a chunk [a, a + n), raw: rows behind n and pieces behind the head's end are read from places that exist, and put
-    // right by `mend` when they are used.  Offsets of a lane are 32-bit, from a base that the wave shares.
-    frag nq[NT][KS], nk[TT][KS], nv[TT][VS];
+    // ---- loads of a chunk [a, a + n): rows behind n are outside of the window and read as zeros; pieces behind the head's end are read
+    // from places that exist, and put right by `mend` when they are used.  Neighbouring lanes take neighbouring pieces of a row: the L1
+    // serves a line a cycle, and in the operands' own order, a row a lane, it served four times as many.
+    constexpr int PK = DKP / V, RK = 64 / PK, NK = C / RK;  // pieces of a row of K, rows that a load takes, loads
+    constexpr int PV = DVS / V, RV = 64 / PV, NV = C / RV;
+    constexpr int KP = Y::KW / V;                           // pieces of a group of contraction slots: four
+    frag sq[NK], sk[NK], sv[NV];
     const unsigned q_t = (unsigned)(S.q_t * sizeof(T)), k_t = (unsigned)(S.k_t * sizeof(T)), v_t = (unsigned)(S.v_t * sizeof(T));
-    const unsigned in_row = V * g * sizeof(T);
-    unsigned qo[NT], ko[TT], vo[TT];
+    const unsigned o_t = (unsigned)(S.o_t * sizeof(T));
+    const unsigned row_k = DK * sizeof(T), row_v = (DV < DVS ? DV : DVS) * sizeof(T);
+    const int rk = lane / PK, pk = lane % PK, rv = lane / PV, pv = lane % PV;
+    auto in_row = [&](int p, int dim) {                     // where in its row a lane reads: its piece, or the row's last 16 bytes
+        if constexpr (WHOLE) return (unsigned)(p * 16);
+        const int last = dim - V;
+        return last < 0 ? 0u : (unsigned)((p * V < last ? p * V : last) * sizeof(T));
+    };
+    const unsigned qo = rk * q_t + in_row(pk, DK), ko = rk * k_t + in_row(pk, DK), vo = rv * v_t + in_row(pv, DV);
+    auto piece = [&](window w, unsigned off, int dim) {
+        if (WHOLE || dim >= V) return __builtin_bit_cast(frag, __builtin_amdgcn_raw_buffer_load_b128(w, off, 0, 0));
+        frag f;                                             // heads of a few elements
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) qo[nt] = (16 * nt + m) * q_t;
-#pragma unroll
-    for (int t = 0; t < TT; ++t) { ko[t] = Y::tile_row(t, m) * k_t; vo[t] = Y::tile_row(t, m) * v_t; }
-    auto piece = [&](const char *base, unsigned row, int p, int dim) {
-        frag f;
-        if constexpr (WHOLE) {
-            __builtin_memcpy(&f, base + (row + in_row) + p * (int)(Y::KW * sizeof(T)), 16);
-        } else if (dim >= V) {
-            const int d = p * Y::KW + V * g, last = dim - V;
-            __builtin_memcpy(&f, base + (row + (unsigned)((d < last ? d : last) * sizeof(T))), 16);
-        } else {                                            // heads of a few elements
-            const T *r = (const T *)(base + row);
-#pragma unroll
-            for (int e = 0; e < V; ++e) f[e] = r[e < dim ? e : 0];
+        for (int e = 0; e < V; ++e) {
+            const unsigned at = off + (e < dim ? e : 0) * sizeof(T);
+            if constexpr (sizeof(T) == 2) f[e] = __builtin_bit_cast(T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(w, at, 0, 0));
+            else f[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(w, at, 0, 0));
         }
         return f;
     };
-    auto mend = [&](frag &f, bool row_is, int p, int dim) {
-        if constexpr (!WHOLE) {
-            const int d = p * Y::KW + V * g, last = dim - V;
-            if (dim % V != 0) {
-                if (dim >= V) f = behind(f, d > last ? d - last : 0);
-                else
+    auto mend = [&](frag &f, int p, int dim) {
+        const int d = p * V, last = dim - V;
+        if (dim % V != 0) {
+            if (dim >= V) f = behind(f, d > last ? d - last : 0);
+            else
 #pragma unroll
-                    for (int e = 0; e < V; ++e) f[e] = d + e < dim ? f[e] : (T)0.f;
-            }
-            row_is = row_is && d < dim;
+                for (int e = 0; e < V; ++e) f[e] = d + e < dim ? f[e] : (T)0.f;
         }
         const u4 u = __builtin_bit_cast(u4, f);
-        f = __builtin_bit_cast(frag, row_is ? u : u4{0u, 0u, 0u, 0u});
+        f = __builtin_bit_cast(frag, d < dim ? u : u4{0u, 0u, 0u, 0u});
     };
-    auto load_q = [&](int a, int n) {
+    auto load = [&](int a, int n) {
+        const unsigned last = n - 1;
+        const window kw = window_of(K + (long long)a * S.k_t, last * k_t + row_k), vw = window_of(Vp + (long long)a * S.v_t, last * v_t + row_v);
+#pragma unroll
+        for (int i = 0; i < NK; ++i) sk[i] = piece(kw, ko + i * RK * k_t, DK);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) sv[i] = piece(vw, vo + i * RV * v_t, DV);
         if constexpr (!STATE_ONLY) {
-            const char *base = (const char *)(Q + (long long)a * S.q_t);
+            const window qw = window_of(Q + (long long)a * S.q_t, last * q_t + row_k);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) nq[nt][ks] = piece(base, 16 * nt + m < n ? qo[nt] : 0u, ks, DK);
+            for (int i = 0; i < NK; ++i) sq[i] = piece(qw, qo + i * RK * q_t, DK);
         }
     };
-    auto load_kv = [&](int a, int n) {
-        const char *kb = (const char *)(K + (long long)a * S.k_t), *vb = (const char *)(Vp + (long long)a * S.v_t);
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            const bool is = Y::tile_row(t, m) < n;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) nk[t][ks] = piece(kb, is ? ko[t] : 0u, ks, DK);
-#pragma unroll
-            for (int vs = 0; vs < VS; ++vs) nv[t][vs] = piece(vb, is ? vo[t] : 0u, vs, DV);
-        }
+    // The starts of 64 tokens are one load and one mask; chunks do not cross their borders (`left`).
+    int block = -1, asked = -1;                             // of the piece: tokens tok_a + 64 block ..; the block that `byte` is of
+    unsigned long long flags = 0;
+    uint8_t byte = 0;
+    auto ask = [&](int k) {
+        asked = k;
+        const int t = tok_a + 64 * k + lane;
+        byte = k >= 0 && t < tok_e ? St[(long long)t * A.a.starts_t] : 0;
     };
-    auto mend_all = [&](int n) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            if constexpr (!STATE_ONLY) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mend(nq[nt][ks], 16 * nt + m < n, ks, DK);
-            }
-#pragma unroll
-            for (int t = 0; t < TT; ++t) mend(nk[t][ks], Y::tile_row(t, m) < n, ks, DK);
+    auto starts_of = [&](int a, int n) -> unsigned {
+        const int k = (a - tok_a) >> 6;
+        if (k != block) {
+            if (asked != k) ask(k);
+            flags = __ballot(byte != 0);
+            block = k;
+            ask(rev ? k - 1 : k + 1);                       // in flight until its chunks come
         }
-#pragma unroll
-        for (int vs = 0; vs < VS; ++vs)
-#pragma unroll
-            for (int t = 0; t < TT; ++t) mend(nv[t][vs], Y::tile_row(t, m) < n, vs, DV);
+        return (unsigned)(flags >> ((a - tok_a) & 63)) & ((2u << (n - 1)) - 1u);
     };
-    uint8_t nflag = 0;
-    auto load_flags = [&](int a, int n) { nflag = St && lane < n ? St[(long long)(a + lane) * A.a.starts_t] : 0; };
 
     bool any_start = false;
     int pos = rev ? tok_e : tok_a, most = C;
-    auto left = [&]() { const int l = rev ? pos - tok_a : tok_e - pos; return l < most ? l : most; };
-    int n = left();
-    if (n > 0) { const int a = rev ? pos - n : pos; load_kv(a, n); load_q(a, n); load_flags(a, n); }
-    while (n > 0) {
-        by_length(n);
-        const int a = rev ? pos - n : pos, pos0 = pos;
-        const unsigned mask = St ? (unsigned)__ballot(nflag != 0) : 0u;
-        // (the starts of a chunk as bits: x and y are of one episode if no bit lies behind the earlier and up to the later)
-        const unsigned upto_last = (2u << (n - 1)) - 1u;
-        if (!WHOLE || n < C) mend_all(n);
-        wave_sync();                                     // the chunk before has been read
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            const int y = Y::tile_row(t, m);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) *(frag *)(ldsK + y * (DKP + Y::PAD) + ks * Y::KW + V * g) = nk[t][ks];
-#pragma unroll
-            for (int vs = 0; vs < VS; ++vs) *(frag *)(ldsV + y * (DVS + Y::PAD) + vs * Y::KW + V * g) = nv[t][vs];
-        }
-        wave_sync();
-        // A value that is not finite would reach other tokens through a weight of zero (0 x NaN).  Such a chunk is taken token by
-        // token instead, where no token shares a product with another.  The check sums the operands on the matrix cores.
+    // (up to the next multiple of C: the first chunk of a reverse scan is the short one, and so is what follows tokens taken singly)
+    auto left = [&]() {
+        const int in = (pos - tok_a) & (C - 1), room = rev ? (in ? in : C) : C - in, l = rev ? pos - tok_a : tok_e - pos;
+        const int n = room < most ? room : most;
+        return l < n ? l : n;
+    };
+    // A turn of the loop writes the chunk that has been loaded to LDS, asks for the next, and computes the first.
+    int a = 0, n = 0;                                       // the chunk in hand: [a, a + n); none in the first turn
+    for (;;) {
+        const bool have = n > 0;
         float z = 0.f;
+        if (have) {
+            if constexpr (!WHOLE) {
+#pragma unroll
+                for (int i = 0; i < NK; ++i) {
+                    mend(sk[i], pk, DK);
+                    if constexpr (!STATE_ONLY) mend(sq[i], pk, DK);
+                }
+#pragma unroll
+                for (int i = 0; i < NV; ++i) mend(sv[i], pv, DV);
+            }
+        // A value that is not finite would reach other tokens through a weight of zero (0 x NaN).  Such a chunk is taken token by
+        // token instead, where no token shares a product with another.  The check sums K and V on the matrix cores.
         if constexpr (TT == 2) {
             f4 z0 = {0.f, 0.f, 0.f, 0.f}, z1 = z0;
             frag one;
 #pragma unroll
             for (int e = 0; e < V; ++e) one[e] = (T)1.f;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) { z0 = Y::mfma(one, nk[0][ks], z0); z1 = Y::mfma(one, nk[1][ks], z1); }
+            for (int i = 0; i < NK; ++i) z0 = Y::mfma(one, sk[i], z0);
 #pragma unroll
-            for (int vs = 0; vs < VS; ++vs) { z0 = Y::mfma(one, nv[0][vs], z0); z1 = Y::mfma(one, nv[1][vs], z1); }
+            for (int i = 0; i < NV; ++i) z1 = Y::mfma(one, sv[i], z1);
             z = z0[0] * 0.f + z1[0] * 0.f;
         } else {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) z = __builtin_fmaf((float)nk[0][ks][e], 0.f, z);
+                for (int i = 0; i < NK; ++i) z = __builtin_fmaf((float)sk[i][e], 0.f, z);
 #pragma unroll
-                for (int vs = 0; vs < VS; ++vs) z = __builtin_fmaf((float)nv[0][vs][e], 0.f, z);
+                for (int i = 0; i < NV; ++i) z = __builtin_fmaf((float)sv[i][e], 0.f, z);
             }
+        }
+        wave_sync();                                     // the chunk before has been read
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            *(frag *)(ldsK + Y::template at<DKP>(i * RK + rk, pk)) = sk[i];
+            if constexpr (!STATE_ONLY) *(frag *)(ldsQ + Y::template at_rows<DKP>(i * RK + rk, pk)) = sq[i];
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) *(frag *)(ldsV + Y::template at<DVS>(i * RV + rv, pv)) = sv[i];
+        wave_sync();
+        }
+        const int pos0 = pos;
+        pos += rev ? -n : n;
+        most = have ? C : most;
+        const int n2 = __builtin_amdgcn_readfirstlane(left()), a2 = __builtin_amdgcn_readfirstlane(rev ? pos - n2 : pos);
+        if (n2 > 0) load(a2, n2);
+        if (!have) {
+            if (n2 <= 0) break;
+            a = a2;
+            n = n2;
+            continue;
+        }
+        by_length(n);
+        const unsigned mask = St ? starts_of(a, n) : 0u;
+        // (starts in the chunk: x and y are of one episode if none lies behind the earlier and up to the later)
+        const int start0 = mask ? __builtin_ctz(mask) : 32, start1 = mask ? 31 - __builtin_clz(mask) : 0;      // the first and the last of them
+        float w[V], reach[NT];                              // wy and rx within the episodes
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] = wy[e];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) reach[nt] = rx[nt];
+        if (mask) {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (rev ? V * g + e >= start0 : V * g + e < start1) w[e] = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                if (rev ? 16 * nt + m < start1 : 16 * nt + m >= start0) reach[nt] = 0.f;
         }
         frag p[NT];
         if constexpr (!STATE_ONLY) {
+            f4 at[NT][TT];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                f4 at[TT];
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int t = 0; t < TT; ++t) at[nt][t] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                frag q[NT];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) q[nt] = *(const frag *)(ldsQ + Y::template at_rows<DKP>(16 * nt + m, KP * ks + g));
 #pragma unroll
                 for (int t = 0; t < TT; ++t) {
-                    at[t] = f4{0.f, 0.f, 0.f, 0.f};
+                    const frag k = *(const frag *)(ldsK + Y::template at<DKP>(Y::tile_row(t, m), KP * ks + g));
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) at[t] = Y::mfma(nk[t][ks], nq[nt][ks], at[t]);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float w = dw[nt][t][r];
-                        if (mask) {
-                            const int x = 16 * nt + m, y = V * g + 4 * t + r;
-                            const unsigned bits = ((2u << x) - 1u) ^ ((2u << y) - 1u);   // the tokens behind one, up to the other
-                            w = (mask & bits) == 0 ? w : 0.f;
-                        }
-                        at[t][r] = mul_or_zero(at[t][r], w);
-                    }
+                    for (int nt = 0; nt < NT; ++nt) at[nt][t] = Y::mfma(k, q[nt], at[nt][t]);
                 }
-                p[nt] = Y::operand(at);
             }
+            if (mask) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    // the lane's column x sees the tokens from <= y < to
+                    const int x = 16 * nt + (here(lane) & 15);
+                    const unsigned upto = (2u << x) - 1u, before = mask & upto, after = mask & ~upto;
+                    const int from = (before && !rev ? 31 - __builtin_clz(before) : 0) - V * g, to = (after && rev ? __builtin_ctz(after) : 32) - V * g;
+#pragma unroll
+                    for (int t = 0; t < TT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) at[nt][t][r] = mul_or_zero(at[nt][t][r], 4 * t + r >= from && 4 * t + r < to ? dw[nt][t][r] : 0.f);
+                }
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int t = 0; t < TT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) at[nt][t][r] = mul_or_zero(at[nt][t][r], dw[nt][t][r]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) p[nt] = Y::operand(at[nt]);
         }
+        phase();
         frag vf[NJ];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) vf[j] = Y::template column<DVS>(ldsV, Y::KW * (j / TT), j % TT, m, g);
-        // the next chunk's loads are in flight while this one is computed
-        pos += rev ? -n : n;
-        most = C;
-        const int n2 = left(), a2 = rev ? pos - n2 : pos;
-        if (n2 > 0) load_kv(a2, n2);
+        for (int j = 0; j < NJ; ++j) vf[j] = Y::template column<DVS>(ldsV, j, m, g);
         f4 o[VS][NT][TT];
         if constexpr (!STATE_ONLY) {
             // P and S as operands are rounded to the inputs' type: 2^-9 of each term at bf16, as much as the output's own rounding; the
             // sums are fp32
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) o[j / TT][nt][j % TT] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
+            for (int ks = 0; ks < KS; ++ks) {
+                frag q[NT];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) q[nt] = *(const frag *)(ldsQ + Y::template at_rows<DKP>(16 * nt + m, KP * ks + g));
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
                     f4 rows[TT];
 #pragma unroll
                     for (int tt = 0; tt < TT; ++tt) rows[tt] = s[ks * TT + tt][j];
                     const frag sf = Y::operand(rows);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) o[j / TT][nt][j % TT] = Y::mfma(sf, nq[nt][ks], o[j / TT][nt][j % TT]);
+                    for (int nt = 0; nt < NT; ++nt) o[j / TT][nt][j % TT] = Y::mfma(sf, q[nt], o[j / TT][nt][j % TT]);
                 }
             }
         }
-        if (n2 > 0) { load_q(a2, n2); load_flags(a2, n2); }
         if constexpr (!STATE_ONLY) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float reach = rx[nt];
-                if (mask) {
-                    const unsigned upto = (2u << (16 * nt + m)) - 1u;
-                    reach = (rev ? mask & upto_last & ~upto : mask & upto) == 0 ? reach : 0.f;
-                }
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     f4 &t = o[j / TT][nt][j % TT];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) t[r] = mul_or_zero(t[r], reach);
+                    for (int r = 0; r < 4; ++r) t[r] = mul_or_zero(t[r], reach[nt]);
                     t = Y::mfma(vf[j], p[nt], t);
                 }
-            }
         }
         if (n > 1 && __any(z != 0.f || z != z)) {
             pos = pos0;
-            most = n = 1;
-            const int a1 = rev ? pos - 1 : pos;
-            load_kv(a1, 1); load_q(a1, 1); load_flags(a1, 1);
+            most = 1;
+            n = 0;                                          // (the next turn only loads)
             continue;
         }
         if constexpr (!STATE_ONLY) {
+            const window ow = window_of(O + (long long)a * S.o_t, (unsigned)(n - 1) * o_t + row_v);
+            auto put = [&](frag f, unsigned off, int p) {
+                if (WHOLE || p * V + V <= DV) {
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, f), ow, off + p * 16, 0, 0);
+                } else {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const int x = 16 * nt + m;
-                if (x < n) {
-                    T *row = O + (long long)(a + x) * S.o_t;
-#pragma unroll
-                    for (int jg = 0; jg < VS; ++jg) {
-                        const frag f = Y::operand(o[jg][nt]);
-                        if constexpr (WHOLE) __builtin_memcpy(row + jg * Y::KW + V * g, &f, 16);
-                        else store_row<T>(row, jg * Y::KW + V * g, DV, f);
-                    }
+                    for (int e = 0; e < V; ++e)
+                        if (p * V + e < DV) {
+                            const T x = f[e];
+                            if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, x), ow, off + p * 16 + 2 * e, 0, 0);
+                            else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), ow, off + p * 16 + 4 * e, 0, 0);
+                        }
                 }
+            };
+            if constexpr (PV <= 4 && NT == 1) {
+                put(Y::operand(o[0][0]), m * o_t, g);
+            } else {                                        // through LDS, so that neighbouring lanes store neighbouring pieces of a row
+                wave_sync();
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int jg = 0; jg < VS; ++jg) *(frag *)(ldsQ + Y::template at_rows<DVS>(16 * nt + m, KP * jg + g)) = Y::operand(o[jg][nt]);
+                wave_sync();
+#pragma unroll
+                for (int i = 0; i < NV; ++i) put(*(const frag *)(ldsQ + Y::template at_rows<DVS>(i * RV + rv, pv)), (unsigned)(i * RV + rv) * o_t, pv);
             }
         }
         // ---- the state behind the chunk
-        float w[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            w[e] = wy[e];
-            if (mask) {
-                const unsigned upto = (2u << ((V * g + e) & 31)) - 1u;
-                if ((rev ? mask & upto : mask & upto_last & ~upto) != 0) w[e] = 0.f;
-            }
-        }
-        const bool fresh = (mask & upto_last) != 0;
+        phase();
+        const bool fresh = mask != 0;
         any_start = any_start || fresh;
         const float gs = fresh ? 0.f : gn;
 #pragma unroll
@@ -427,18 +519,35 @@ void seq_scan_kernel(const Args A) {
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s[i][j][r] = mul_or_zero(s[i][j][r], gs);
-        frag kt[NI];
+        if constexpr (NI <= 4) {                            // (K's columns: held, or with heads of 128 read again for each of V's)
+            frag kt[NI];
 #pragma unroll
-        for (int i = 0; i < NI; ++i) kt[i] = Y::template column<DKP>(ldsK, Y::KW * (i / TT), i % TT, m, g);
+            for (int i = 0; i < NI; ++i) kt[i] = Y::template column<DKP>(ldsK, i, m, g);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            frag part[Y::PARTS];
-            Y::weighted(vf[j], w, part);
+            for (int j = 0; j < NJ; ++j) {
+                frag part[PARTS];
+                Y::template weighted<PARTS>(vf[j], w, part);
 #pragma unroll
-            for (int pp = 0; pp < Y::PARTS; ++pp)
+                for (int pp = 0; pp < PARTS; ++pp)
 #pragma unroll
-                for (int i = 0; i < NI; ++i) s[i][j] = Y::mfma(kt[i], part[pp], s[i][j]);
+                    for (int i = 0; i < NI; ++i) s[i][j] = Y::mfma(kt[i], part[pp], s[i][j]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                frag part[PARTS];
+                Y::template weighted<PARTS>(vf[j], w, part);
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    const frag kt = Y::template column<DKP>(ldsK, i, m, g);
+#pragma unroll
+                    for (int pp = 0; pp < PARTS; ++pp) s[i][j] = Y::mfma(kt, part[pp], s[i][j]);
+                }
+                phase();
+            }
         }
+        if (n2 <= 0) break;
+        a = a2;
         n = n2;
     }
 
@@ -448,7 +557,7 @@ void seq_scan_kernel(const Args A) {
 #pragma unroll
             for (int j = 0; j < NJ; ++j) *(f4 *)(ws + (i * NJ + j) * 256) = s[i][j];
         if (lane == 0 && strip == 0)
-            A.carry[((long long)sc * A.a.B * A.a.H + bh) * nseg + seg] = any_start ? -1.f : power(lg, tok_e - tok_a);
+            A.carry[((long long)sc * A.a.B * A.a.H + bh) * nseg + seg] = any_start ? 0.f : power(lg, tok_e - tok_a);
     } else {
         // rows at and behind the length
         for (int t = tok_e + g; t < seg_e; t += 4)
@@ -462,16 +571,10 @@ void seq_scan_kernel(const Args A) {
                     store_row<T>(O + (long long)t * S.o_t, jg * Y::KW + V * u, DV, z);
                 }
         if ((rev ? seg == 0 : seg == nseg - 1) && S.s_out) {
-            float *p = S.s_out + b * S.s_b + h * S.s_h;
-#pragma unroll
-            for (int i = 0; i < NI; ++i)
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int dk = Y::KW * (i / TT) + Y::tile_row(i % TT, 4 * g + r), dv = Y::KW * (j / TT) + Y::tile_row(j % TT, m);
-                        if (dk < DK && dv < DV) p[dk * S.s_k + (dv0 + dv) * S.s_v] = s[i][j][r];
-                    }
+            const gbytes_out p = shared_base_out(S.s_out + b * S.s_b + h * S.s_h);
+            state_elements([&](int i, int j, int r, bool is, unsigned at) {
+                if (is) *(__attribute__((address_space(1))) float *)(p + at) = s[i][j][r];
+            });
         }
     }
 }
@@ -509,14 +612,17 @@ template <typename T, int DKP, int DVS> __global__ __launch_bounds__(256) void s
         const f4 u = *p;
         const float c = carry[seg];
         *p = s;
-        s = c < 0.f ? u : s * c + u;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = mul_or_zero(s[r], c) + u[r];
     }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
 int padded(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
 
-// One kernel per pair of padded sizes.  The state of a wave is dkp x dvs: 64 x 64 at most, 128 x 32 where dk needs 128.
+// Strips are 64 value columns (32 where dk needs 128: the state has to fit the registers) if that makes a wave for every SIMD, and else
+// the narrowest that fill a tile: each wave then has less to do for a chunk, and K, Q and their products are repeated.  Measured: 64
+// windows of 160 x 4 heads of 64, fp32, forward 35 us wide (256 waves), 20 us narrow (1024 waves).
 struct Plan { int dkp, dvs, n_sib, sib0[PVDER_SEQ_MAX_SCANS + 1]; };
 
 bool plan_of(const pvder_seq_attn *a, Plan &P) {
@@ -530,15 +636,18 @@ bool plan_of(const pvder_seq_attn *a, Plan &P) {
         dv = s.dv > dv ? s.dv : dv;
     }
     P.dkp = padded(dk);
-    P.dvs = padded(dv);
-    if (P.dvs > 64) P.dvs = 64;
-    if (P.dkp == 128) P.dvs = 32;
-    P.n_sib = 0;
-    for (int i = 0; i < a->n_scans; ++i) {
-        P.sib0[i] = P.n_sib;
-        P.n_sib += (a->scan[i].dv + P.dvs - 1) / P.dvs;
+    const int widest = padded(dv) < 64 && P.dkp < 128 ? padded(dv) : (P.dkp == 128 ? 32 : 64), narrowest = a->dtype == PVDER_SEQ_BF16 ? 32 : 16;
+    for (const int dvs : {widest, narrowest}) {
+        P.dvs = dvs;
+        P.n_sib = 0;
+        for (int i = 0; i < a->n_scans; ++i) {
+            const int strips = (a->scan[i].dv + dvs - 1) / dvs;
+            P.sib0[i] = P.n_sib;
+            P.n_sib += strips;
+        }
+        for (int i = a->n_scans; i <= PVDER_SEQ_MAX_SCANS; ++i) P.sib0[i] = P.n_sib;
+        if ((long long)a->B * a->H * P.n_sib >= 1024) break;
     }
-    for (int i = a->n_scans; i <= PVDER_SEQ_MAX_SCANS; ++i) P.sib0[i] = P.n_sib;
     return true;
 }
 
@@ -547,29 +656,36 @@ int seg_len_of(const pvder_seq_attn *a) {
     return (per + c - 1) / c * c;
 }
 
-template <typename T, int DKP, int DVS, bool WHOLE> int launch(const Args &A, hipStream_t st) {
-    const long long blocks = (A.n_groups + 7) / 8 * 8 * A.n_sib;
+template <typename T, int DKP, int DVS, bool WHOLE> int launch(const Args &A, const Plan &P, hipStream_t st) {
+    constexpr int MOST = sizeof(T) == 2 ? 3 : 1, LEAST = sizeof(T) == 2 ? 2 : 1;
+    const long long blocks = (A.n_groups + 7ll) / 8 * 8 * A.n_sib;
     if (blocks > 0x7fffffffll) return kEinval;
+    const dim3 grid((unsigned)blocks), block(64);
+    const int bytes = tile_bytes<T>(DKP, DVS);
+    bool state = false;
+    for (int i = 0; i < A.a.n_scans; ++i) state = state || A.a.scan[i].s_out != nullptr;
     if (A.a.segments > 1) {
-        seq_scan_kernel<T, DKP, DVS, WHOLE, true><<<dim3((unsigned)blocks), dim3(64), 0, st>>>(A);
+        seq_scan_kernel<T, DKP, DVS, WHOLE, true, MOST><<<grid, block, bytes, st>>>(A);
         const long long items = (long long)A.a.B * A.a.H * A.n_sib * (DKP * DVS / 4);
         seq_join_kernel<T, DKP, DVS><<<dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st>>>(A);
     }
-    seq_scan_kernel<T, DKP, DVS, WHOLE, false><<<dim3((unsigned)blocks), dim3(64), 0, st>>>(A);
+    if (state) seq_scan_kernel<T, DKP, DVS, WHOLE, false, MOST><<<grid, block, bytes, st>>>(A);
+    else seq_scan_kernel<T, DKP, DVS, WHOLE, false, LEAST><<<grid, block, bytes, st>>>(A);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : -(int)e;
 }
 
-template <typename T, int DKP, int DVS> int fit(const Args &A, hipStream_t st) {
+template <typename T, int DKP, int DVS> int fit(const Args &A, const Plan &P, hipStream_t st) {
     bool whole = true;
     for (int i = 0; i < A.a.n_scans; ++i) whole = whole && A.a.scan[i].dk == DKP && A.a.scan[i].dv % DVS == 0;
-    return whole ? launch<T, DKP, DVS, true>(A, st) : launch<T, DKP, DVS, false>(A, st);
+    return whole ? launch<T, DKP, DVS, true>(A, P, st) : launch<T, DKP, DVS, false>(A, P, st);
 }
 
 template <typename T> int pick(const Args &A, const Plan &P, hipStream_t st) {
-    if (P.dkp == 32) return P.dvs == 32 ? fit<T, 32, 32>(A, st) : fit<T, 32, 64>(A, st);
-    if (P.dkp == 64) return P.dvs == 32 ? fit<T, 64, 32>(A, st) : fit<T, 64, 64>(A, st);
-    return fit<T, 128, 32>(A, st);
+    constexpr int NARROW = sizeof(T) == 2 ? 32 : 16;
+    if (P.dkp == 32) return P.dvs == 64 ? fit<T, 32, 64>(A, P, st) : (P.dvs == 32 ? fit<T, 32, 32>(A, P, st) : fit<T, 32, NARROW>(A, P, st));
+    if (P.dkp == 64) return P.dvs == 64 ? fit<T, 64, 64>(A, P, st) : (P.dvs == 32 ? fit<T, 64, 32>(A, P, st) : fit<T, 64, NARROW>(A, P, st));
+    return P.dvs == 32 ? fit<T, 128, 32>(A, P, st) : fit<T, 128, NARROW>(A, P, st);
 }
 
 }  // namespace
@@ -599,8 +715,10 @@ extern "C" int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream) {
         {
             const pvder_seq_scan &s = a->scan[i];
             if (!s.q || !s.k || !s.v || !s.o) return kEinval;
+            if ((s.s_in || s.s_out) && (s.s_k < 0 || s.s_v < 0 || (s.dk * s.s_k + s.dv * s.s_v) >= (1ll << 29))) return kEinval;
             const int64_t most = PVDER_SEQ_MAX_TOKEN_STRIDE / (a->dtype == PVDER_SEQ_BF16 ? 2 : 4);
-            if (s.q_t < 0 || s.k_t < 0 || s.v_t < 0 || s.q_t > most || s.k_t > most || s.v_t > most) return kEinval;
+            // (a row's end, where the window of a chunk ends, has to lie before the next row)
+            if (s.q_t < s.dk || s.k_t < s.dk || s.v_t < s.dv || s.o_t < s.dv || s.q_t > most || s.k_t > most || s.v_t > most || s.o_t > most) return kEinval;
         }
     if (a->B == 0) return 0;
     A.a = *a;
@@ -608,8 +726,10 @@ extern "C" int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream) {
     A.seg_len = A.a.T ? seg_len_of(&A.a) : 32;
     A.n_sib = P.n_sib;
     for (int i = 0; i <= PVDER_SEQ_MAX_SCANS; ++i) A.sib0[i] = P.sib0[i];
-    A.n_groups = (long long)a->B * a->H * A.a.segments;
+    const long long groups = (long long)a->B * a->H * A.a.segments;
+    if (groups > 0x7fffffffll) return kEinval;
+    A.n_groups = (unsigned)groups;
     A.per_sib = (long long)P.dkp * P.dvs;
-    A.carry = A.a.segments > 1 ? A.a.workspace + A.n_groups * P.n_sib * A.per_sib : nullptr;
+    A.carry = A.a.segments > 1 ? A.a.workspace + groups * P.n_sib * A.per_sib : nullptr;
     return a->dtype == PVDER_SEQ_BF16 ? pick<__bf16>(A, P, (hipStream_t)stream) : pick<float>(A, P, (hipStream_t)stream);
 }

@@ -16,6 +16,27 @@ typedef __bf16 b4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u4 __attribute__((ext_vector_type(4)));
 
+// Global memory as a base that a wave shares (held in scalar registers, and hidden from the compiler's address arithmetic, which would
+// carry an address of 64 bits for every load round a loop) and an offset of each lane, 32 bits.
+typedef const __attribute__((address_space(1))) char *gbytes;
+typedef __attribute__((address_space(1))) char *gbytes_out;
+__device__ __forceinline__ gbytes shared_base(const void *p) {
+    gbytes b = (gbytes)p;
+    asm volatile("" : "+s"(b));
+    return b;
+}
+__device__ __forceinline__ gbytes_out shared_base_out(void *p) {
+    gbytes_out b = (gbytes_out)p;
+    asm volatile("" : "+s"(b));
+    return b;
+}
+
+// Memory of a wave with its end: what lies behind `bytes` reads as zero and is not written, without a branch.
+typedef __amdgpu_buffer_rsrc_t window;
+__device__ __forceinline__ window window_of(const void *p, unsigned bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)bytes, 0x00027000);
+}
+
 template <typename T> struct Vec;
 template <> struct Vec<float> { typedef f4 type; static constexpr int N = 4; };
 template <> struct Vec<__bf16> { typedef b8 type; static constexpr int N = 8; };
@@ -68,8 +89,8 @@ template <typename T> __device__ __forceinline__ void store_row(T *row, int d, i
 extern "C" __device__ float pvder_seq_mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
 __device__ __forceinline__ float mul_or_zero(float a, float b) { return pvder_seq_mul_legacy(a, b); }
 
-// g^n of a decay given as its base-2 logarithm lg <= 0; g^0 = 1 also where lg is -infinity
-__device__ __forceinline__ float power(float lg, int n) { return n == 0 ? 1.f : exp2f(lg * (float)n); }
+// g^n of a decay given as its base-2 logarithm lg <= 0, zero where it would be no normal number; g^0 = 1 also where lg is -infinity
+__device__ __forceinline__ float power(float lg, int n) { return __builtin_amdgcn_exp2f(n == 0 ? 0.f : lg * (float)n); }
 // log_decay as the kernels take it: growth and NaN count as no decay
 __device__ __forceinline__ float log2_decay(float log_decay) { return (log_decay < 0.f ? log_decay : 0.f) * 1.44269504088896340736f; }
 

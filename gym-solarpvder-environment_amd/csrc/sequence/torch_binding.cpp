@@ -45,10 +45,11 @@ bool wants_grad(Maybe t) { return has(t) && t->requires_grad(); }
 
 // unit stride in the last dimension (a copy only where it has another)
 Tensor rows(const Tensor &t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
-// and tokens near enough for the kernels' 32-bit offsets within a chunk
+// and tokens that lie behind each other (not on each other, as in an expanded tensor) and near enough for 32-bit offsets within a chunk
 Tensor tokens(const Tensor &t) {
     const Tensor r = rows(t);
-    return r.stride(1) * (int64_t)r.element_size() <= PVDER_SEQ_MAX_TOKEN_STRIDE ? r : r.contiguous();
+    const int64_t st = r.stride(1);
+    return r.size(1) <= 1 || (st >= r.size(3) && st * (int64_t)r.element_size() <= PVDER_SEQ_MAX_TOKEN_STRIDE) ? r : r.contiguous();
 }
 
 struct Heads { int64_t H, DK, DV; };
@@ -87,6 +88,11 @@ void check_flags(Maybe t, at::IntArrayRef shape) {
 }
 
 // ---- decay attention over windows -------------------------------------------------------------------------------------------
+// a state whose matrices are dense (rows or columns first)
+Tensor dense(const Tensor &s) {
+    const int64_t k = s.size(2), v = s.size(3);
+    return (s.stride(3) == 1 && s.stride(2) == v) || (s.stride(2) == 1 && s.stride(3) == k) ? s : s.contiguous();
+}
 struct State { int64_t b, h, k, v; };
 State state_strides(Maybe t, const Heads &d) {
     if (has(t)) return {t->stride(0), t->stride(1), t->stride(2), t->stride(3)};
@@ -97,10 +103,11 @@ pvder_seq_scan scan_of(const Tensor &q, const Tensor &k, const Tensor &v, const 
                        float a_write, float a_intra, bool reverse) {
     pvder_seq_scan c;
     c.q = q.data_ptr(); c.k = k.data_ptr(); c.v = v.data_ptr(); c.o = o.data_ptr();
-    c.q_b = q.stride(0); c.q_t = q.stride(1); c.q_h = q.stride(2);
-    c.k_b = k.stride(0); c.k_t = k.stride(1); c.k_h = k.stride(2);
-    c.v_b = v.stride(0); c.v_t = v.stride(1); c.v_h = v.stride(2);
-    c.o_b = o.stride(0); c.o_t = o.stride(1); c.o_h = o.stride(2);
+    const bool many = q.size(1) > 1;                       // (the stride of a single token says nothing: a row's length)
+    c.q_b = q.stride(0); c.q_t = many ? q.stride(1) : q.size(3); c.q_h = q.stride(2);
+    c.k_b = k.stride(0); c.k_t = many ? k.stride(1) : k.size(3); c.k_h = k.stride(2);
+    c.v_b = v.stride(0); c.v_t = many ? v.stride(1) : v.size(3); c.v_h = v.stride(2);
+    c.o_b = o.stride(0); c.o_t = many ? o.stride(1) : o.size(3); c.o_h = o.stride(2);
     c.s_in = (const float *)s_in; c.s_out = (float *)s_out;
     c.s_b = s.b; c.s_h = s.h; c.s_k = s.k; c.s_v = s.v;
     c.a_read = a_read; c.a_write = a_write; c.a_intra = a_intra;
@@ -202,16 +209,16 @@ struct DecayAttention : torch::autograd::Function<DecayAttention> {
     }
 };
 
-py::object decay_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &log_decay, optional<double> scale_, Maybe initial,
+py::object decay_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &log_decay, optional<double> scale_, Maybe initial_,
                            Maybe starts, Maybe lengths, bool want_state) {
     const Heads d = check_qkv(q_, k_, v_, log_decay, 4, "[B, T, H, D]");
     const int64_t B = q_.size(0), T = q_.size(1);
-    same_device(q_, initial, "initial_state");
+    same_device(q_, initial_, "initial_state");
     same_device(q_, starts, "starts");
     same_device(q_, lengths, "lengths");
-    if (has(initial)) {
-        NEED_TYPE(initial->scalar_type() == at::kFloat, "initial_state must be float32");
-        const at::IntArrayRef is = initial->sizes();
+    if (has(initial_)) {
+        NEED_TYPE(initial_->scalar_type() == at::kFloat, "initial_state must be float32");
+        const at::IntArrayRef is = initial_->sizes();
         NEED(is.size() == 4 && is[0] == B && is[1] == d.H && is[2] == d.DK && is[3] == d.DV, "initial_state must be [", B, ", ", d.H, ", ", d.DK, ", ", d.DV, "]: got ", is);
     }
     check_flags(starts, {B, T});
@@ -222,6 +229,7 @@ py::object decay_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_,
     const float scale = scale_of(scale_, d.DK);
     on_gpu(q_, "q");
     const Tensor q = tokens(q_), k = tokens(k_), v = tokens(v_);
+    const optional<Tensor> initial = has(initial_) ? optional<Tensor>(dense(*initial_)) : optional<Tensor>();
     Tensor out, final;
     if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v) || wants_grad(initial))) {
         const auto r = DecayAttention::apply(q, k, v, log_decay, initial, starts, lengths, (double)scale, want_state);

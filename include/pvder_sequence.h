@@ -24,10 +24,10 @@ enum { PVDER_SEQ_MAX_HEAD = 128, PVDER_SEQ_MAX_SCANS = 3, PVDER_SEQ_MAX_WIDTH = 
 typedef struct pvder_seq_scan {
     const void *q, *k, *v;          /* [B, T, H, dk], [B, T, H, dk], [B, T, H, dv] */
     void *o;                        /* [B, T, H, dv]; rows at and behind lengths[b] are written as zeros */
-    int64_t q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h, o_b, o_t, o_h;   /* q_t, k_t, v_t: 0 .. PVDER_SEQ_MAX_TOKEN_STRIDE bytes */
+    int64_t q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h, o_b, o_t, o_h;   /* q_t .. o_t: a row's length .. PVDER_SEQ_MAX_TOKEN_STRIDE bytes */
     const float *s_in;              /* state that comes in, NULL: zeros; element (i, j) of (b, h) at b s_b + h s_h + i s_k + j s_v */
     float *s_out;                   /* state that goes out, NULL: not wanted; same strides */
-    int64_t s_b, s_h, s_k, s_v;
+    int64_t s_b, s_h, s_k, s_v;     /* s_k, s_v >= 0, dk s_k + dv s_v < 2^29 */
     float a_read, a_write, a_intra;
     int32_t dk, dv, reverse;
 } pvder_seq_scan;

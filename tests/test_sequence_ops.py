@@ -113,7 +113,9 @@ def test_norm_refuses():
 def _attn(**tail):
     scan = dict(dk=8, dv=8)
     scan.update({k: tail.pop(k) for k in list(tail) if k in scan})
-    one = SCAN.pack(*([64] * 4), *([0] * 12), 0, 0, *([0] * 4), 1.0, 1.0, 1.0, scan["dk"], scan["dv"], 0)
+    row = max(scan["dk"], scan["dv"], 1) if tail.get("apart", True) else 0
+    tail.pop("apart", None)
+    one = SCAN.pack(*([64] * 4), *([0, row, 0] * 4), 0, 0, *([0] * 4), 1.0, 1.0, 1.0, scan["dk"], scan["dv"], 0)
     d = dict(decay=64, work=0, B=1, T=8, H=1, n=1, dtype=0, segments=1)
     d.update(tail)
     return ctypes.create_string_buffer(one * 3 + ATTN_TAIL.pack(d["decay"], 0, 0, d["work"], 0, 0, d["B"], d["T"], d["H"], d["n"], d["dtype"], d["segments"]))
@@ -127,6 +129,7 @@ def test_c_entries_refuse_before_any_launch():
         assert L.pvder_seq_attn_plan(_attn(**bad)) == _native.EINVAL, bad
         assert L.pvder_seq_attn_run(_attn(**bad), None) == _native.EINVAL, bad
     assert L.pvder_seq_attn_run(_attn(decay=0), None) == _native.EINVAL
+    assert L.pvder_seq_attn_run(_attn(apart=False), None) == _native.EINVAL              # tokens on top of each other
     assert L.pvder_seq_attn_run(_attn(segments=0), None) == _native.EINVAL
     assert L.pvder_seq_attn_run(_attn(segments=2), None) == _native.EINVAL          # no workspace
     assert L.pvder_seq_attn_run(_attn(segments=2, work=68), None) == _native.EINVAL  # a workspace that is not aligned
