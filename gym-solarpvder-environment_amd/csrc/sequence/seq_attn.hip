@@ -239,9 +239,10 @@ void seq_scan_kernel(const Args A) {
         gn = power(lg, n);
     };
 
-    // ---- loads of a chunk [a, a + n): rows behind n are outside of the window and read as zeros; pieces behind the head's end are read
-    // from places that exist, and put right by `mend` when they are used.  Neighbouring lanes take neighbouring pieces of a row: the L1
-    // serves a line a cycle, and in the operands' own order, a row a lane, it served four times as many.
+    // ---- loads of a chunk [a, a + n): rows behind n and pieces behind the head's end are outside of the window and read as zeros; the
+    // piece that the head's end cuts is read from 16 bytes before that end, and shifted by `mend` when it is used.  Neighbouring lanes
+    // take neighbouring pieces of a row: the L1 serves a line a cycle, and in the operands' own order, a row a lane, it served four times
+    // as many.
     constexpr int PK = DKP / V, RK = 64 / PK, NK = C / RK;  // pieces of a row of K, rows that a load takes, loads
     constexpr int PV = DVS / V, RV = 64 / PV, NV = C / RV;
     constexpr int KP = Y::KW / V;                           // pieces of a group of contraction slots: four
@@ -250,10 +251,11 @@ void seq_scan_kernel(const Args A) {
     const unsigned o_t = (unsigned)(S.o_t * sizeof(T));
     const unsigned row_k = DK * sizeof(T), row_v = (DV < DVS ? DV : DVS) * sizeof(T);
     const int rk = lane / PK, pk = lane % PK, rv = lane / PV, pv = lane % PV;
-    auto in_row = [&](int p, int dim) {                     // where in its row a lane reads: its piece, or the row's last 16 bytes
+    constexpr unsigned OUTSIDE = 0x80000000u;               // of every window, whatever rows are added
+    auto in_row = [&](int p, int dim) {
         if constexpr (WHOLE) return (unsigned)(p * 16);
-        const int last = dim - V;
-        return last < 0 ? 0u : (unsigned)((p * V < last ? p * V : last) * sizeof(T));
+        if (p * V >= dim) return OUTSIDE;
+        return (unsigned)((dim < V || p * V <= dim - V ? p * V : dim - V) * sizeof(T));
     };
     const unsigned qo = rk * q_t + in_row(pk, DK), ko = rk * k_t + in_row(pk, DK), vo = rv * v_t + in_row(pv, DV);
     auto piece = [&](window w, unsigned off, int dim) {
@@ -261,22 +263,15 @@ void seq_scan_kernel(const Args A) {
         frag f;                                             // heads of a few elements
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const unsigned at = off + (e < dim ? e : 0) * sizeof(T);
+            const unsigned at = e < dim ? off + e * (unsigned)sizeof(T) : OUTSIDE;
             if constexpr (sizeof(T) == 2) f[e] = __builtin_bit_cast(T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(w, at, 0, 0));
             else f[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(w, at, 0, 0));
         }
         return f;
     };
+    const bool ragged = !WHOLE && (DK % V != 0 || S.dv % V != 0);
     auto mend = [&](frag &f, int p, int dim) {
-        const int d = p * V, last = dim - V;
-        if (dim % V != 0) {
-            if (dim >= V) f = behind(f, d > last ? d - last : 0);
-            else
-#pragma unroll
-                for (int e = 0; e < V; ++e) f[e] = d + e < dim ? f[e] : (T)0.f;
-        }
-        const u4 u = __builtin_bit_cast(u4, f);
-        f = __builtin_bit_cast(frag, d < dim ? u : u4{0u, 0u, 0u, 0u});
+        if (dim > V) f = behind(f, p * V < dim && p * V > dim - V ? p * V - (dim - V) : 0);
     };
     auto load = [&](int a, int n) {
         const unsigned last = n - 1;
@@ -325,7 +320,7 @@ void seq_scan_kernel(const Args A) {
         const bool have = n > 0;
         float z = 0.f;
         if (have) {
-            if constexpr (!WHOLE) {
+            if (ragged) {
 #pragma unroll
                 for (int i = 0; i < NK; ++i) {
                     mend(sk[i], pk, DK);
@@ -483,7 +478,9 @@ void seq_scan_kernel(const Args A) {
         if constexpr (!STATE_ONLY) {
             const window ow = window_of(O + (long long)a * S.o_t, (unsigned)(n - 1) * o_t + row_v);
             auto put = [&](frag f, unsigned off, int p) {
-                if (WHOLE || p * V + V <= DV) {
+                if (!ragged) {
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, f), ow, WHOLE || p * V < DV ? off + p * 16 : OUTSIDE, 0, 0);
+                } else if (p * V + V <= DV) {
                     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, f), ow, off + p * 16, 0, 0);
                 } else {
 #pragma unroll
@@ -606,14 +603,23 @@ template <typename T, int DKP, int DVS> __global__ __launch_bounds__(256) void s
     }
     const float *carry = A.carry + ((long long)sc * A.a.B * A.a.H + bh) * nseg;
     float *ws = A.a.workspace + at * 4;
-    for (int n = 0; n < nseg; ++n) {
-        const int seg = rev ? nseg - 1 - n : n;
-        f4 *p = (f4 *)(ws + ((bh * nseg + seg) * A.n_sib + sib) * A.per_sib);
-        const f4 u = *p;
-        const float c = carry[seg];
-        *p = s;
+    auto place = [&](int n) { return (f4 *)(ws + (((long long)bh * nseg + (rev ? nseg - 1 - n : n)) * A.n_sib + sib) * A.per_sib); };
+    for (int n0 = 0; n0 < nseg; n0 += 8) {                 // eight pieces' loads are in flight together
+        f4 u[8];
+        float c[8];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[r] = mul_or_zero(s[r], c) + u[r];
+        for (int k = 0; k < 8; ++k) {
+            const int n = n0 + k < nseg ? n0 + k : nseg - 1;
+            u[k] = *place(n);
+            c[k] = carry[rev ? nseg - 1 - n : n];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (n0 + k >= nseg) break;
+            *place(n0 + k) = s;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[r] = mul_or_zero(s[r], c[k]) + u[k][r];
+        }
     }
 }
 
