@@ -154,7 +154,7 @@ void seq_scan_kernel(const Args A) {
     const int seg = (int)(grp - bh * (unsigned)nseg), b = (int)(bh / (unsigned)A.a.H), h = (int)(bh - (unsigned)b * (unsigned)A.a.H);
     const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
     const bool rev = S.reverse != 0;
-    const int DK = S.dk, DV = S.dv - dv0;                 // columns of this strip's rows that exist: dv0 .. dv0 + DV
+    const int DK = S.dk, DV = S.dv - dv0;                 // columns of this strip that exist, and of those behind it
 
     int len = A.a.T;
     if (A.a.lengths) { len = A.a.lengths[b]; len = len < 0 ? 0 : (len > A.a.T ? A.a.T : len); }
@@ -167,8 +167,8 @@ void seq_scan_kernel(const Args A) {
 
     const T *Q = (const T *)S.q + b * S.q_b + h * S.q_h;
     const T *K = (const T *)S.k + b * S.k_b + h * S.k_h;
-    const T *Vp = (const T *)S.v + b * S.v_b + h * S.v_h + dv0;
-    T *O = (T *)S.o + b * S.o_b + h * S.o_h + dv0;
+    const T *Vp = (const T *)S.v + b * S.v_b + h * S.v_h;
+    T *O = (T *)S.o + b * S.o_b + h * S.o_h;
     const uint8_t *St = A.a.starts ? A.a.starts + b * A.a.starts_b : nullptr;
 
     const float lg = log2_decay(A.a.log_decay[h]);
@@ -249,41 +249,29 @@ void seq_scan_kernel(const Args A) {
     frag sq[NK], sk[NK], sv[NV];
     const unsigned q_t = (unsigned)(S.q_t * sizeof(T)), k_t = (unsigned)(S.k_t * sizeof(T)), v_t = (unsigned)(S.v_t * sizeof(T));
     const unsigned o_t = (unsigned)(S.o_t * sizeof(T));
-    const unsigned row_k = DK * sizeof(T), row_v = (DV < DVS ? DV : DVS) * sizeof(T);
+    const unsigned row_k = DK * sizeof(T), row_v = S.dv * sizeof(T);
     const int rk = lane / PK, pk = lane % PK, rv = lane / PV, pv = lane % PV;
     constexpr unsigned OUTSIDE = 0x80000000u;               // of every window, whatever rows are added
-    auto in_row = [&](int p, int dim) {
-        if constexpr (WHOLE) return (unsigned)(p * 16);
-        if (p * V >= dim) return OUTSIDE;
-        return (unsigned)((dim < V || p * V <= dim - V ? p * V : dim - V) * sizeof(T));
+    auto in_row = [&](int d, int dim) {                     // the bytes of elements d .. d + V of a row of dim
+        if (!WHOLE && d >= dim) return OUTSIDE;
+        return (unsigned)((WHOLE || d <= dim - V ? d : dim - V) * sizeof(T));
     };
-    const unsigned qo = rk * q_t + in_row(pk, DK), ko = rk * k_t + in_row(pk, DK), vo = rv * v_t + in_row(pv, DV);
-    auto piece = [&](window w, unsigned off, int dim) {
-        if (WHOLE || dim >= V) return __builtin_bit_cast(frag, __builtin_amdgcn_raw_buffer_load_b128(w, off, 0, 0));
-        frag f;                                             // heads of a few elements
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const unsigned at = e < dim ? off + e * (unsigned)sizeof(T) : OUTSIDE;
-            if constexpr (sizeof(T) == 2) f[e] = __builtin_bit_cast(T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(w, at, 0, 0));
-            else f[e] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(w, at, 0, 0));
-        }
-        return f;
-    };
+    const int dk0 = pk * V, dvp = dv0 + pv * V;             // the first elements of a lane's pieces
+    const unsigned qo = rk * q_t + in_row(dk0, DK), ko = rk * k_t + in_row(dk0, DK), vo = rv * v_t + in_row(dvp, S.dv);
+    auto piece = [&](window w, unsigned off) { return __builtin_bit_cast(frag, __builtin_amdgcn_raw_buffer_load_b128(w, off, 0, 0)); };
     const bool ragged = !WHOLE && (DK % V != 0 || S.dv % V != 0);
-    auto mend = [&](frag &f, int p, int dim) {
-        if (dim > V) f = behind(f, p * V < dim && p * V > dim - V ? p * V - (dim - V) : 0);
-    };
+    auto mend = [&](frag &f, int d, int dim) { f = behind(f, d < dim && d > dim - V ? d - (dim - V) : 0); };
     auto load = [&](int a, int n) {
         const unsigned last = n - 1;
         const window kw = window_of(K + (long long)a * S.k_t, last * k_t + row_k), vw = window_of(Vp + (long long)a * S.v_t, last * v_t + row_v);
 #pragma unroll
-        for (int i = 0; i < NK; ++i) sk[i] = piece(kw, ko + i * RK * k_t, DK);
+        for (int i = 0; i < NK; ++i) sk[i] = piece(kw, ko + i * RK * k_t);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) sv[i] = piece(vw, vo + i * RV * v_t, DV);
+        for (int i = 0; i < NV; ++i) sv[i] = piece(vw, vo + i * RV * v_t);
         if constexpr (!STATE_ONLY) {
             const window qw = window_of(Q + (long long)a * S.q_t, last * q_t + row_k);
 #pragma unroll
-            for (int i = 0; i < NK; ++i) sq[i] = piece(qw, qo + i * RK * q_t, DK);
+            for (int i = 0; i < NK; ++i) sq[i] = piece(qw, qo + i * RK * q_t);
         }
     };
     // The starts of 64 tokens are one load and one mask; chunks do not cross their borders (`left`).
@@ -315,6 +303,7 @@ void seq_scan_kernel(const Args A) {
         return l < n ? l : n;
     };
     // A turn of the loop writes the chunk that has been loaded to LDS, asks for the next, and computes the first.
+    if (St && left() > 0) ask(rev ? (tok_e - 1 - tok_a) >> 6 : 0);
     int a = 0, n = 0;                                       // the chunk in hand: [a, a + n); none in the first turn
     for (;;) {
         const bool have = n > 0;
@@ -323,11 +312,11 @@ void seq_scan_kernel(const Args A) {
             if (ragged) {
 #pragma unroll
                 for (int i = 0; i < NK; ++i) {
-                    mend(sk[i], pk, DK);
-                    if constexpr (!STATE_ONLY) mend(sq[i], pk, DK);
+                    mend(sk[i], dk0, DK);
+                    if constexpr (!STATE_ONLY) mend(sq[i], dk0, DK);
                 }
 #pragma unroll
-                for (int i = 0; i < NV; ++i) mend(sv[i], pv, DV);
+                for (int i = 0; i < NV; ++i) mend(sv[i], dvp, S.dv);
             }
         // A value that is not finite would reach other tokens through a weight of zero (0 x NaN).  Such a chunk is taken token by
         // token instead, where no token shares a product with another.  The check sums K and V on the matrix cores.
@@ -477,23 +466,22 @@ void seq_scan_kernel(const Args A) {
         }
         if constexpr (!STATE_ONLY) {
             const window ow = window_of(O + (long long)a * S.o_t, (unsigned)(n - 1) * o_t + row_v);
-            auto put = [&](frag f, unsigned off, int p) {
-                if (!ragged) {
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, f), ow, WHOLE || p * V < DV ? off + p * 16 : OUTSIDE, 0, 0);
-                } else if (p * V + V <= DV) {
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, f), ow, off + p * 16, 0, 0);
+            auto put = [&](frag f, unsigned off, int d) {   // elements d .. of a row
+                if (!ragged || d + V <= S.dv) {
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, f), ow, WHOLE || d < S.dv ? off + d * (unsigned)sizeof(T) : OUTSIDE, 0, 0);
                 } else {
 #pragma unroll
                     for (int e = 0; e < V; ++e)
-                        if (p * V + e < DV) {
+                        if (d + e < S.dv) {
                             const T x = f[e];
-                            if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, x), ow, off + p * 16 + 2 * e, 0, 0);
-                            else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), ow, off + p * 16 + 4 * e, 0, 0);
+                            const unsigned at = off + (d + e) * (unsigned)sizeof(T);
+                            if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, x), ow, at, 0, 0);
+                            else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), ow, at, 0, 0);
                         }
                 }
             };
             if constexpr (PV <= 4 && NT == 1) {
-                put(Y::operand(o[0][0]), m * o_t, g);
+                put(Y::operand(o[0][0]), m * o_t, dv0 + g * V);
             } else {                                        // through LDS, so that neighbouring lanes store neighbouring pieces of a row
                 wave_sync();
 #pragma unroll
@@ -502,7 +490,7 @@ void seq_scan_kernel(const Args A) {
                     for (int jg = 0; jg < VS; ++jg) *(frag *)(ldsQ + Y::template at_rows<DVS>(16 * nt + m, KP * jg + g)) = Y::operand(o[jg][nt]);
                 wave_sync();
 #pragma unroll
-                for (int i = 0; i < NV; ++i) put(*(const frag *)(ldsQ + Y::template at_rows<DVS>(i * RV + rv, pv)), (unsigned)(i * RV + rv) * o_t, pv);
+                for (int i = 0; i < NV; ++i) put(*(const frag *)(ldsQ + Y::template at_rows<DVS>(i * RV + rv, pv)), (unsigned)(i * RV + rv) * o_t, dvp);
             }
         }
         // ---- the state behind the chunk
@@ -557,16 +545,12 @@ void seq_scan_kernel(const Args A) {
             A.carry[((long long)sc * A.a.B * A.a.H + bh) * nseg + seg] = any_start ? 0.f : power(lg, tok_e - tok_a);
     } else {
         // rows at and behind the length
-        for (int t = tok_e + g; t < seg_e; t += 4)
+        for (int t = tok_e + rv; t < seg_e; t += RV) {
+            T *row = O + (long long)t * S.o_t;
 #pragma unroll
-            for (int jg = 0; jg < VS; ++jg)
-#pragma unroll
-                for (int u = m; u < Y::KW / V; u += 16) {
-                    frag z;
-#pragma unroll
-                    for (int e = 0; e < V; ++e) z[e] = (T)0.f;
-                    store_row<T>(O + (long long)t * S.o_t, jg * Y::KW + V * u, DV, z);
-                }
+            for (int e = 0; e < V; ++e)
+                if (dvp + e < S.dv) row[dvp + e] = (T)0.f;
+        }
         if ((rev ? seg == 0 : seg == nseg - 1) && S.s_out) {
             const gbytes_out p = shared_base_out(S.s_out + b * S.s_b + h * S.s_h);
             state_elements([&](int i, int j, int r, bool is, unsigned at) {
@@ -634,10 +618,11 @@ struct Plan { int dkp, dvs, n_sib, sib0[PVDER_SEQ_MAX_SCANS + 1]; };
 bool plan_of(const pvder_seq_attn *a, Plan &P) {
     if (!a || a->n_scans < 1 || a->n_scans > PVDER_SEQ_MAX_SCANS || a->B < 0 || a->T < 0 || a->H < 1) return false;
     if (a->dtype != PVDER_SEQ_F32 && a->dtype != PVDER_SEQ_BF16) return false;
+    const int least = a->dtype == PVDER_SEQ_BF16 ? 8 : 4;  // 16 bytes: the kernels read rows in such pieces
     int dk = 0, dv = 0;
     for (int i = 0; i < a->n_scans; ++i) {
         const pvder_seq_scan &s = a->scan[i];
-        if (s.dk < 1 || s.dv < 1 || s.dk > PVDER_SEQ_MAX_HEAD || s.dv > PVDER_SEQ_MAX_HEAD) return false;
+        if (s.dk < least || s.dv < least || s.dk > PVDER_SEQ_MAX_HEAD || s.dv > PVDER_SEQ_MAX_HEAD) return false;
         dk = s.dk > dk ? s.dk : dk;
         dv = s.dv > dv ? s.dv : dv;
     }
@@ -699,12 +684,14 @@ template <typename T> int pick(const Args &A, const Plan &P, hipStream_t st) {
 extern "C" int64_t pvder_seq_attn_plan(pvder_seq_attn *a) {
     Plan P;
     if (!plan_of(a, P)) return kEinval;
+    // Pieces of T side by side cost a second reading of K and V, a state of each piece in memory and two more launches: worth it where
+    // the waves leave most of the card idle and the pieces make up for it.  Measured at heads of 64, bf16, one piece against the rule's:
+    // 16 waves of 2048 tokens 82 us and 22 (32 pieces), 128 waves 84 and 35 (8); 512 waves 86 and 100 (4), 1024 waves of 512 61 and 86 (2).
     const long long waves = (long long)a->B * a->H * P.n_sib;
     a->segments = 1;
-    if (waves >= 1 && a->T >= 256) {
-        const long long want = 2048 / waves, most = a->T / 128;
-        const long long n = want < most ? want : most;
-        a->segments = n < 2 ? 1 : (int32_t)n;
+    if (waves >= 1 && waves <= 384 && a->T >= 384) {
+        const long long want = 2048 / waves, most = a->T / 64, n = want < most ? want : most;
+        if (n >= 4) a->segments = (int32_t)n;
     }
     if (a->segments == 1) return 0;
     const int64_t bhs = (int64_t)a->B * a->H * a->segments;

@@ -228,6 +228,19 @@ py::object decay_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_,
     }
     const float scale = scale_of(scale_, d.DK);
     on_gpu(q_, "q");
+    const int64_t least = 16 / (int64_t)q_.element_size();
+    if (d.DK < least || d.DV < least) {
+        // heads of less than 16 bytes: with zeros behind them, and without them again
+        const int64_t k0 = d.DK < least ? least - d.DK : 0, v0 = d.DV < least ? least - d.DV : 0;
+        optional<Tensor> s0;
+        if (has(initial_)) s0 = at::constant_pad_nd(*initial_, {0, v0, 0, k0});
+        const py::object r = decay_attention(at::constant_pad_nd(q_, {0, k0}), at::constant_pad_nd(k_, {0, k0}), at::constant_pad_nd(v_, {0, v0}), log_decay,
+                                             (double)scale, s0, starts, lengths, want_state);
+        auto cut = [&](const py::handle &o) { return o.cast<Tensor>().narrow(-1, 0, d.DV); };
+        if (!want_state) return py::cast(cut(r));
+        const py::tuple both = r.cast<py::tuple>();
+        return py::make_tuple(cut(both[0]), cut(both[1]).narrow(2, 0, d.DK));
+    }
     const Tensor q = tokens(q_), k = tokens(k_), v = tokens(v_);
     const optional<Tensor> initial = has(initial_) ? optional<Tensor>(dense(*initial_)) : optional<Tensor>();
     Tensor out, final;

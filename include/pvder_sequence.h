@@ -29,7 +29,7 @@ typedef struct pvder_seq_scan {
     float *s_out;                   /* state that goes out, NULL: not wanted; same strides */
     int64_t s_b, s_h, s_k, s_v;     /* s_k, s_v >= 0, dk s_k + dv s_v < 2^29 */
     float a_read, a_write, a_intra;
-    int32_t dk, dv, reverse;
+    int32_t dk, dv, reverse;        /* dk, dv: 16 bytes of elements (8 bf16, 4 fp32) .. PVDER_SEQ_MAX_HEAD */
 } pvder_seq_scan;
 
 typedef struct pvder_seq_attn {

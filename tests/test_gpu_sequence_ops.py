@@ -60,7 +60,7 @@ def _run(ops, c, scale=None, train=True):
 # one token, one partial chunk, whole chunks, one token over, head sizes that fill no tile, every padded size, several pieces of T
 SHAPES = [(1, 1, 1, 1, 1), (2, 1, 3, 16, 32), (2, 5, 3, 16, 16), (1, 16, 1, 32, 32), (1, 32, 2, 32, 64), (3, 33, 2, 24, 40), (1, 65, 1, 64, 64),
           (2, 160, 4, 64, 64), (2, 70, 1, 65, 128), (1, 131, 2, 128, 33), (1, 255, 1, 128, 128), (1, 256, 1, 7, 3), (2, 300, 1, 100, 20),
-          (1, 1000, 2, 20, 64), (1, 700, 1, 128, 127)]
+          (1, 1000, 2, 20, 64), (1, 700, 1, 128, 127), (1, 600, 1, 7, 3), (1, 450, 3, 64, 64), (3, 400, 2, 36, 65)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
