@@ -615,31 +615,48 @@ int padded(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
 // windows of 160 x 4 heads of 64, fp32, forward 35 us wide (256 waves), 20 us narrow (1024 waves).
 struct Plan { int dkp, dvs, n_sib, sib0[PVDER_SEQ_MAX_SCANS + 1]; };
 
-bool plan_of(const pvder_seq_attn *a, Plan &P) {
+bool valid(const pvder_seq_attn *a) {
     if (!a || a->n_scans < 1 || a->n_scans > PVDER_SEQ_MAX_SCANS || a->B < 0 || a->T < 0 || a->H < 1) return false;
     if (a->dtype != PVDER_SEQ_F32 && a->dtype != PVDER_SEQ_BF16) return false;
     const int least = a->dtype == PVDER_SEQ_BF16 ? 8 : 4;  // 16 bytes: the kernels read rows in such pieces
-    int dk = 0, dv = 0;
     for (int i = 0; i < a->n_scans; ++i) {
         const pvder_seq_scan &s = a->scan[i];
         if (s.dk < least || s.dv < least || s.dk > PVDER_SEQ_MAX_HEAD || s.dv > PVDER_SEQ_MAX_HEAD) return false;
-        dk = s.dk > dk ? s.dk : dk;
-        dv = s.dv > dv ? s.dv : dv;
     }
-    P.dkp = padded(dk);
-    const int widest = padded(dv) < 64 && P.dkp < 128 ? padded(dv) : (P.dkp == 128 ? 32 : 64), narrowest = a->dtype == PVDER_SEQ_BF16 ? 32 : 16;
+    return true;
+}
+
+// The scans of `a` whose dk has the padded size dkp, as an argument of their own: scans of other sizes would be padded to the largest.
+int of_size(const pvder_seq_attn *a, int dkp, pvder_seq_attn &sub) {
+    sub = *a;
+    sub.n_scans = 0;
+    for (int i = 0; i < a->n_scans; ++i)
+        if (padded(a->scan[i].dk) == dkp) sub.scan[sub.n_scans++] = a->scan[i];
+    return sub.n_scans;
+}
+
+Plan plan_of(const pvder_seq_attn *a, int dkp) {
+    Plan P;
+    int dv = 0;
+    for (int i = 0; i < a->n_scans; ++i) dv = a->scan[i].dv > dv ? a->scan[i].dv : dv;
+    P.dkp = dkp;
+    const int widest = padded(dv) < 64 && dkp < 128 ? padded(dv) : (dkp == 128 ? 32 : 64), narrowest = a->dtype == PVDER_SEQ_BF16 ? 32 : 16;
     for (const int dvs : {widest, narrowest}) {
         P.dvs = dvs;
         P.n_sib = 0;
         for (int i = 0; i < a->n_scans; ++i) {
-            const int strips = (a->scan[i].dv + dvs - 1) / dvs;
             P.sib0[i] = P.n_sib;
-            P.n_sib += strips;
+            P.n_sib += (a->scan[i].dv + dvs - 1) / dvs;
         }
         for (int i = a->n_scans; i <= PVDER_SEQ_MAX_SCANS; ++i) P.sib0[i] = P.n_sib;
         if ((long long)a->B * a->H * P.n_sib >= 1024) break;
     }
-    return true;
+    return P;
+}
+
+int64_t workspace_of(const pvder_seq_attn *a, const Plan &P) {
+    const int64_t bhs = (int64_t)a->B * a->H * a->segments;
+    return (bhs * P.n_sib * P.dkp * P.dvs + bhs * a->n_scans + 3) / 4 * 4;      // (whole 16 bytes: the next size's begins there)
 }
 
 int seg_len_of(const pvder_seq_attn *a) {
@@ -682,47 +699,57 @@ template <typename T> int pick(const Args &A, const Plan &P, hipStream_t st) {
 }  // namespace
 
 extern "C" int64_t pvder_seq_attn_plan(pvder_seq_attn *a) {
-    Plan P;
-    if (!plan_of(a, P)) return kEinval;
+    if (!valid(a)) return kEinval;
     // Pieces of T side by side cost a second reading of K and V, a state of each piece in memory and two more launches: worth it where
     // the waves leave most of the card idle and the pieces make up for it.  Measured at heads of 64, bf16, one piece against the rule's:
     // 16 waves of 2048 tokens 82 us and 22 (32 pieces), 128 waves 84 and 35 (8); 512 waves 86 and 100 (4), 1024 waves of 512 61 and 86 (2).
-    const long long waves = (long long)a->B * a->H * P.n_sib;
+    pvder_seq_attn sub;
+    long long waves = 0;
+    for (const int dkp : {32, 64, 128})
+        if (of_size(a, dkp, sub)) waves += (long long)a->B * a->H * plan_of(&sub, dkp).n_sib;
     a->segments = 1;
     if (waves >= 1 && waves <= 384 && a->T >= 384) {
         const long long want = 2048 / waves, most = a->T / 64, n = want < most ? want : most;
         if (n >= 4) a->segments = (int32_t)n;
     }
     if (a->segments == 1) return 0;
-    const int64_t bhs = (int64_t)a->B * a->H * a->segments;
-    return bhs * P.n_sib * P.dkp * P.dvs + bhs * a->n_scans;
+    int64_t floats = 0;
+    for (const int dkp : {32, 64, 128})
+        if (of_size(a, dkp, sub)) floats += workspace_of(&sub, plan_of(&sub, dkp));
+    return floats;
 }
 
 extern "C" int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream) {
-    Args A;
-    Plan P;
-    if (!plan_of(a, P) || a->segments < 1 || !a->log_decay) return kEinval;
+    if (!valid(a) || a->segments < 1 || !a->log_decay) return kEinval;
     if (a->segments > 1 && (!a->workspace || ((uintptr_t)a->workspace & 15))) return kEinval;
-    if (a->B > 0 && a->T > 0)
-        for (int i = 0; i < a->n_scans; ++i)
-        {
+    if ((long long)a->B * a->H * a->segments > 0x7fffffffll) return kEinval;
+    if (a->B > 0 && a->T > 0) {
+        const int64_t most = PVDER_SEQ_MAX_TOKEN_STRIDE / (a->dtype == PVDER_SEQ_BF16 ? 2 : 4);
+        for (int i = 0; i < a->n_scans; ++i) {
             const pvder_seq_scan &s = a->scan[i];
             if (!s.q || !s.k || !s.v || !s.o) return kEinval;
             if ((s.s_in || s.s_out) && (s.s_k < 0 || s.s_v < 0 || (s.dk * s.s_k + s.dv * s.s_v) >= (1ll << 29))) return kEinval;
-            const int64_t most = PVDER_SEQ_MAX_TOKEN_STRIDE / (a->dtype == PVDER_SEQ_BF16 ? 2 : 4);
             // (a row's end, where the window of a chunk ends, has to lie before the next row)
             if (s.q_t < s.dk || s.k_t < s.dk || s.v_t < s.dv || s.o_t < s.dv || s.q_t > most || s.k_t > most || s.v_t > most || s.o_t > most) return kEinval;
         }
+    }
     if (a->B == 0) return 0;
-    A.a = *a;
-    if (A.a.T == 0) A.a.segments = 1;
-    A.seg_len = A.a.T ? seg_len_of(&A.a) : 32;
-    A.n_sib = P.n_sib;
-    for (int i = 0; i <= PVDER_SEQ_MAX_SCANS; ++i) A.sib0[i] = P.sib0[i];
-    const long long groups = (long long)a->B * a->H * A.a.segments;
-    if (groups > 0x7fffffffll) return kEinval;
-    A.n_groups = (unsigned)groups;
-    A.per_sib = (long long)P.dkp * P.dvs;
-    A.carry = A.a.segments > 1 ? A.a.workspace + groups * P.n_sib * A.per_sib : nullptr;
-    return a->dtype == PVDER_SEQ_BF16 ? pick<__bf16>(A, P, (hipStream_t)stream) : pick<float>(A, P, (hipStream_t)stream);
+    float *work = a->workspace;
+    for (const int dkp : {32, 64, 128}) {
+        Args A;
+        if (!of_size(a, dkp, A.a)) continue;
+        if (A.a.T == 0) A.a.segments = 1;
+        const Plan P = plan_of(&A.a, dkp);
+        A.seg_len = A.a.T ? seg_len_of(&A.a) : 32;
+        A.n_sib = P.n_sib;
+        for (int i = 0; i <= PVDER_SEQ_MAX_SCANS; ++i) A.sib0[i] = P.sib0[i];
+        A.n_groups = (unsigned)((long long)a->B * a->H * A.a.segments);
+        A.per_sib = (long long)P.dkp * P.dvs;
+        A.a.workspace = work;
+        A.carry = A.a.segments > 1 ? work + (long long)A.n_groups * P.n_sib * A.per_sib : nullptr;
+        if (A.a.segments > 1) work += workspace_of(&A.a, P);
+        const int rc = a->dtype == PVDER_SEQ_BF16 ? pick<__bf16>(A, P, (hipStream_t)stream) : pick<float>(A, P, (hipStream_t)stream);
+        if (rc) return rc;
+    }
+    return 0;
 }
