@@ -75,6 +75,12 @@ template <bool EVEN, typename T, int TPR, int NV> __device__ __forceinline__ voi
         }
 }
 
+// what stands before is finished before what stands behind begins: keeps the weights of one vector in registers at a time
+__device__ __forceinline__ void apart() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // sum over the TPR lanes of a row; TPR > 64: over the whole block (every lane of it calls)
 template <int TPR> __device__ __forceinline__ float row_sum(float x, float *lds) {
 #pragma unroll
@@ -146,13 +152,14 @@ template <typename T, int TPR, int NV, bool EVEN> __global__ __launch_bounds__(b
     __shared__ float lds[TPR > 64 ? TPR / 64 : 1];
     __shared__ float sums[RPB > 1 ? RPB * TPR * E : 1];
     const int t = threadIdx.x % TPR, D = a.width, grp = threadIdx.x / TPR;
-    Row<T, NV> post, pre, scale, gpost, gpre, gscale;
-    auto weights = [&]() {
-        load_param<EVEN, T, TPR, NV>(post, a.post, t, D, 1.f);
-        load_param<EVEN, T, TPR, NV>(pre, a.pre, t, D, 1.f);
-        load_param<EVEN, T, TPR, NV>(scale, a.scale, t, D, 1.f);
+    Row<T, NV> gpost, gpre, gscale;
+    Row<T, LEAN ? 1 : NV> post, pre, scale;                // (LEAN: those of one vector at a time)
+    auto weights = [&](int i) {
+        load_param<EVEN, T, TPR, LEAN ? 1 : NV>(post, a.post, i * TPR + t, D, 1.f);
+        load_param<EVEN, T, TPR, LEAN ? 1 : NV>(pre, a.pre, i * TPR + t, D, 1.f);
+        load_param<EVEN, T, TPR, LEAN ? 1 : NV>(scale, a.scale, i * TPR + t, D, 1.f);
     };
-    if constexpr (!LEAN) weights();
+    if constexpr (!LEAN) weights(0);
 #pragma unroll
     for (int e = 0; e < E; ++e) gpost.e[e] = gpre.e[e] = gscale.e[e] = 0.f;
     const float inv = 1.f / (float)D;
@@ -173,10 +180,10 @@ template <typename T, int TPR, int NV, bool EVEN> __global__ __launch_bounds__(b
         row(dx, a.dx, a.dx_r);
         row(dh, a.dh, a.dh_r);
         const float ry = a.stats[2 * r], rh = a.stats[2 * r + 1];
-        if constexpr (LEAN) weights();
-        Row<T, NV> hn, sg, sc, dn;
-        auto branch = [&](int e) {                          // element e of h', the sigmoid and its derivative
-            const int i = e / V, k = e % V;
+        Row<T, LEAN ? 1 : NV> hn, sg, sc;
+        Row<T, NV> dn;
+        auto branch = [&](int i, int k) {                   // element k of vector i of h', the sigmoid and its derivative
+            const int e = LEAN ? k : i * V + k;
             sg.e[e] = 1.f;
             sc.e[e] = 0.f;
             if (a.gate) sigmoids((float)z[i][k], sg.e[e], sc.e[e]);
@@ -184,28 +191,38 @@ template <typename T, int TPR, int NV, bool EVEN> __global__ __launch_bounds__(b
         };
         float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            branch(e);
-            s = __builtin_fmaf((float)dx[e / V][e % V] * pre.e[e], hn.e[e], s);
+        for (int i = 0; i < NV; ++i) {
+            if constexpr (LEAN) weights(i);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const int e = LEAN ? k : i * V + k;
+                branch(i, k);
+                s = __builtin_fmaf((float)dx[i][k] * pre.e[e], hn.e[e], s);
+            }
+            if constexpr (LEAN) apart();
         }
         const float A = row_sum<TPR>(s, lds) * inv * rh * rh;
-        if constexpr (LEAN) weights();
         s = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int i = e / V, k = e % V;
-            if constexpr (LEAN) branch(e);
-            const float x = (float)dx[i][k], n0 = (float)y[i][k] * ry, n = n0 * post.e[e];
-            const float d = __builtin_fmaf(rh, x * pre.e[e] - hn.e[e] * A, (float)dh[i][k]), du = d * scale.e[e];
-            if (on) {                                      // (a row past the end stands in for the block's first)
-                gpre.e[e] = __builtin_fmaf(x * hn.e[e], rh, gpre.e[e]);
-                gscale.e[e] = __builtin_fmaf(d, n * sg.e[e], gscale.e[e]);
-                gpost.e[e] = __builtin_fmaf(du * sg.e[e], n0, gpost.e[e]);
+        for (int i = 0; i < NV; ++i) {
+            if constexpr (LEAN) weights(i);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const int e = LEAN ? k : i * V + k, x0 = i * V + k;
+                if constexpr (LEAN) branch(i, k);
+                const float x = (float)dx[i][k], n0 = (float)y[i][k] * ry, n = n0 * post.e[e];
+                const float d = __builtin_fmaf(rh, x * pre.e[e] - hn.e[e] * A, (float)dh[i][k]), du = d * scale.e[e];
+                if (on) {                                  // (a row past the end stands in for the block's first)
+                    gpre.e[x0] = __builtin_fmaf(x * hn.e[e], rh, gpre.e[x0]);
+                    gscale.e[x0] = __builtin_fmaf(d, n * sg.e[e], gscale.e[x0]);
+                    gpost.e[x0] = __builtin_fmaf(du * sg.e[e], n0, gpost.e[x0]);
+                }
+                z[i][k] = (T)(sc.e[e] * du * n);
+                dh[i][k] = (T)d;
+                dn.e[x0] = du * sg.e[e] * post.e[e];
+                s = __builtin_fmaf(dn.e[x0], (float)y[i][k], s);
             }
-            z[i][k] = (T)(sc.e[e] * du * n);
-            dh[i][k] = (T)d;
-            dn.e[e] = du * sg.e[e] * post.e[e];
-            s = __builtin_fmaf(dn.e[e], (float)y[i][k], s);
+            if constexpr (LEAN) apart();
         }
         const float B = row_sum<TPR>(s, lds) * inv * ry * ry;
         if (!on) continue;
