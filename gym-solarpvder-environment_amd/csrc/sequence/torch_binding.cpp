@@ -4,6 +4,8 @@
 // against 3 us for a step of one env, 160 us against 77 us for a training pass over 64 windows of 160 steps.
 #include <torch/extension.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <cmath>
 #include <optional>
@@ -152,6 +154,20 @@ std::tuple<Tensor, Tensor> attention_forward(const Tensor &q, const Tensor &k, c
     return {out, final};
 }
 
+// A leaf's gradient accumulator belongs to the stream on which its first graph was recorded, and lives as long as a graph does.  A
+// backward pass that is captured while such a graph of another stream lives would have to wait for that stream, which a capture cannot:
+// torch's engine throws in a thread of its own, and the process ends.  So the forward pass is refused.
+void capturable(const Tensor &t, const char *name) {
+    if (!t.defined() || !t.requires_grad() || t.grad_fn()) return;
+    const auto acc = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!acc) return;
+    const auto own = acc->stream();
+    const c10::Stream now = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).unwrap();
+    TORCH_CHECK(!own || *own == now, name, " is a leaf of a graph that lives on another stream: its backward pass cannot be captured. Delete what holds that graph "
+                "(its outputs, its losses) before the capture.");
+}
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+
 void once() {
     TORCH_CHECK(!at::GradMode::is_enabled(), "the sequence operators are differentiable once: create_graph=True is not supported");
 }
@@ -245,6 +261,12 @@ py::object decay_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_,
     const optional<Tensor> initial = has(initial_) ? optional<Tensor>(dense(*initial_)) : optional<Tensor>();
     Tensor out, final;
     if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v) || wants_grad(initial))) {
+        if (capturing()) {
+            capturable(q_, "q");
+            capturable(k_, "k");
+            capturable(v_, "v");
+            if (has(initial_)) capturable(*initial_, "initial_state");
+        }
         const auto r = DecayAttention::apply(q, k, v, log_decay, initial, starts, lengths, (double)scale, want_state);
         out = r[0];
         if (want_state) final = r[1];
@@ -394,6 +416,12 @@ std::tuple<Tensor, Tensor> gated_residual_norm(const Tensor &h, const Tensor &y,
     NEED(std::isfinite((float)eps) && eps >= 0.0, "eps must be a finite number >= 0");
     on_gpu(h, "residual");
     if (at::GradMode::is_enabled() && (wants_grad(h) || wants_grad(y) || wants_grad(post) || wants_grad(pre) || wants_grad(gate) || wants_grad(scale))) {
+        if (capturing()) {
+            const Tensor *all[] = {&h, &y, &post, &pre, has(gate) ? &*gate : nullptr, has(scale) ? &*scale : nullptr};
+            const char *names[] = {"residual", "y", "post_weight", "pre_weight", "gate", "scale"};
+            for (int i = 0; i < 6; ++i)
+                if (all[i]) capturable(*all[i], names[i]);
+        }
         const auto r = GatedResidualNorm::apply(h, y, post, pre, gate, scale, eps);
         return {r[0], r[1]};
     }

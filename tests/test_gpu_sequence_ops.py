@@ -471,3 +471,31 @@ def test_inputs_changed_before_the_backward_pass_are_noticed(ops, gpu_device):
     ops.decay_attention_step(c["q"][:, 0], c["k"][:, 0], c["v"][:, 0], c["log_decay"], state)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_a_capture_beside_a_living_graph_of_its_leaves_is_refused(ops, gpu_device):
+    """Its backward pass would wait, within a capture, for the other graph's stream: refused in the forward pass, before anything."""
+    c, nc = _case(1, 9, 1, 8, 8, torch.float32, gpu_device), _norm_case(4, 8, torch.float32, gpu_device)
+    q, w = c["q"].detach().requires_grad_(), nc["post"].detach().requires_grad_()
+    out = ops.decay_attention(q, c["k"], c["v"], c["log_decay"])
+    h, x = ops.gated_residual_norm(nc["h"], nc["y"], w, nc["pre"])
+    torch.cuda.synchronize()
+    g, t = torch.cuda.CUDAGraph(), torch.ones(4, device=gpu_device)
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="another stream"):
+            ops.decay_attention(q, c["k"], c["v"], c["log_decay"])
+        with pytest.raises(RuntimeError, match="another stream"):
+            ops.gated_residual_norm(nc["h"], nc["y"], w, nc["pre"])
+        t.mul_(2)
+    want = torch.autograd.grad(out, q, c["do"])[0].clone(), torch.autograd.grad([h, x], w, [nc["dh"], nc["dx"]])[0].clone()
+    del out, h, x
+    g2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g2):
+        out = ops.decay_attention(q, c["k"], c["v"], c["log_decay"])
+        h, x = ops.gated_residual_norm(nc["h"], nc["y"], w, nc["pre"])
+        got = torch.autograd.grad(out, q, c["do"])[0], torch.autograd.grad([h, x], w, [nc["dh"], nc["dx"]])[0]
+    for _ in range(3):
+        g2.replay()
+        t.add_(1)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
