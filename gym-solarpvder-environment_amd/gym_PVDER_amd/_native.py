@@ -10,6 +10,7 @@ import ctypes as C
 import os
 import shutil
 import subprocess
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG_ROOT = os.path.dirname(HERE)                       # gym-solarpvder-environment_amd/
@@ -104,23 +105,27 @@ def hipcc_path() -> str:
     return shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 
 
-def _build(lib_path: str, deps, cmd, force: bool, verbose: bool) -> str:
-    """Run ``cmd`` + the output's name unless ``lib_path`` is newer than everything it is made of."""
-    if (not force and os.path.exists(lib_path)
-            and all(os.path.getmtime(d) <= os.path.getmtime(lib_path) for d in deps)):
-        return lib_path
-    os.makedirs(LIB_DIR, exist_ok=True)
-    tmp = "%s.%d.tmp" % (lib_path, os.getpid())          # build aside, then rename: never a half-written library
-    cmd = cmd + ["-o", tmp]
+def _fresh(lib_path: str, deps) -> bool:
+    """Whether ``lib_path`` is there and newer than everything it is made of."""
+    return os.path.exists(lib_path) and all(os.path.getmtime(d) <= os.path.getmtime(lib_path) for d in deps)
+
+
+def _run(cmd, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd))
+    subprocess.check_call(cmd)
+
+
+def _build(lib_path: str, cmd, verbose: bool) -> None:
+    """Run ``cmd``, which ends in the output's name, aside, then rename: never a half-written library."""
+    os.makedirs(LIB_DIR, exist_ok=True)
+    tmp = "%s.%d.tmp" % (lib_path, os.getpid())
     try:
-        subprocess.check_call(cmd)
+        _run(cmd + ["-o", tmp], verbose)
         os.replace(tmp, lib_path)
     finally:
         if os.path.exists(tmp):
             os.remove(tmp)
-    return lib_path
 
 
 def build_native(force: bool = False, verbose: bool = False) -> str:
@@ -128,7 +133,8 @@ def build_native(force: bool = False, verbose: bool = False) -> str:
     srcs = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(".hip")]
     deps = srcs + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hpp")]
     deps += [os.path.join(INCLUDE, "pvder_hip.h"), os.path.join(INCLUDE, "pvder_agent.h")]
-    _build(LIB_PATH, deps, [hipcc_path()] + HIPCC_FLAGS + ["-fPIC", "-shared", "-I" + INCLUDE, "-I" + CSRC] + srcs, force, verbose)
+    if force or not _fresh(LIB_PATH, deps):
+        _build(LIB_PATH, [hipcc_path()] + HIPCC_FLAGS + ["-fPIC", "-shared", "-I" + INCLUDE, "-I" + CSRC] + srcs, verbose)
     build_sequence(force, verbose)
     return LIB_PATH
 
@@ -136,28 +142,38 @@ def build_native(force: bool = False, verbose: bool = False) -> str:
 def build_sequence(force: bool = False, verbose: bool = False) -> str:
     """Compile csrc/sequence/*.hip for gfx950 into gym_PVDER_amd/lib/libpvder_sequence.so (in-tree), and the torch binding that
     calls it, csrc/sequence/torch_binding.cpp, with the host compiler."""
+    from concurrent.futures import ThreadPoolExecutor
     names = sorted(os.listdir(SEQUENCE_CSRC))
     srcs = [os.path.join(SEQUENCE_CSRC, f) for f in names if f.endswith(".hip")]
     header = os.path.join(INCLUDE, "pvder_sequence.h")
-    deps = srcs + [os.path.join(SEQUENCE_CSRC, f) for f in names if f.endswith(".hpp")] + [header]
-    _build(SEQUENCE_LIB_PATH, deps, [hipcc_path()] + SEQUENCE_HIPCC_FLAGS + ["-fPIC", "-shared", "-I" + INCLUDE] + srcs, force, verbose)
     binding = os.path.join(SEQUENCE_CSRC, "torch_binding.cpp")
-    if (not force and os.path.exists(SEQUENCE_TORCH_PATH)
-            and all(os.path.getmtime(d) <= os.path.getmtime(SEQUENCE_TORCH_PATH) for d in (binding, header))):
+    lib_old = force or not _fresh(SEQUENCE_LIB_PATH, srcs + [os.path.join(SEQUENCE_CSRC, f) for f in names if f.endswith(".hpp")] + [header])
+    torch_old = force or not _fresh(SEQUENCE_TORCH_PATH, [binding, header])
+    if not (lib_old or torch_old):
         return SEQUENCE_LIB_PATH                         # (without importing torch)
-    import sysconfig
-    import torch
-    inc = os.path.join(os.path.dirname(torch.__file__), "include")
-    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
-    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           "-DTORCH_API_INCLUDE_EXTENSION_H", "-DTORCH_EXTENSION_NAME=_pvder_sequence_torch",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
-           "-I" + INCLUDE, "-isystem" + inc, "-isystem" + os.path.join(inc, "torch", "csrc", "api", "include"),
-           "-isystem" + os.path.join(rocm, "include"), "-isystem" + sysconfig.get_paths()["include"], binding,
-           "-L" + LIB_DIR, "-l:libpvder_sequence.so", "-Wl,-rpath,$ORIGIN", "-L" + libs, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip",
-           "-ltorch", "-ltorch_python"]
-    _build(SEQUENCE_TORCH_PATH, [binding, header], cmd, force, verbose)
+    os.makedirs(LIB_DIR, exist_ok=True)
+    with tempfile.TemporaryDirectory(dir=LIB_DIR) as tmp, ThreadPoolExecutor(4) as pool:
+        # every source by itself, side by side, the host compiler's among them; then the links
+        jobs, objs, host = [], [], os.path.join(tmp, "torch_binding.o")
+        if torch_old:
+            import sysconfig
+            import torch
+            inc, libs = (os.path.join(os.path.dirname(torch.__file__), d) for d in ("include", "lib"))
+            rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+            jobs.append(["g++", "-O2", "-std=c++17", "-fPIC", "-c", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_API_INCLUDE_EXTENSION_H",
+                         "-DTORCH_EXTENSION_NAME=_pvder_sequence_torch", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
+                         "-I" + INCLUDE, "-isystem" + inc, "-isystem" + os.path.join(inc, "torch", "csrc", "api", "include"),
+                         "-isystem" + os.path.join(rocm, "include"), "-isystem" + sysconfig.get_paths()["include"], binding, "-o", host])
+        if lib_old:
+            for f in srcs:
+                objs.append(os.path.join(tmp, os.path.basename(f) + ".o"))
+                jobs.append([hipcc_path()] + SEQUENCE_HIPCC_FLAGS + ["-fPIC", "-c", "-I" + INCLUDE, f, "-o", objs[-1]])
+        list(pool.map(lambda cmd: _run(cmd, verbose), jobs))
+        if lib_old:
+            _build(SEQUENCE_LIB_PATH, [hipcc_path(), "--offload-arch=gfx950", "-shared", "-fPIC"] + objs, verbose)
+        if torch_old:
+            _build(SEQUENCE_TORCH_PATH, ["g++", "-shared", host, "-L" + LIB_DIR, "-l:libpvder_sequence.so", "-Wl,-rpath,$ORIGIN", "-L" + libs, "-lc10",
+                                         "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python"], verbose)
     return SEQUENCE_LIB_PATH
 
 
