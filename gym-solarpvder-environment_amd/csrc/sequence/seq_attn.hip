@@ -115,7 +115,7 @@ struct Args {
     int seg_len, n_sib;                     // tokens of a piece; strips of one (b, h, piece), all scans together
     int sib0[PVDER_SEQ_MAX_SCANS + 1];      // first strip of each scan
     unsigned n_groups;                      // (b, h, piece) triples
-    long long per_sib;            // workspace floats of one strip's state
+    long long per_sib;                      // workspace floats of one strip's state
     float *carry;                           // [scan][b][h][piece]: what a piece leaves of the state before it (0 behind a start)
 };
 
@@ -294,6 +294,21 @@ void seq_scan_kernel(const Args A) {
         return (unsigned)(flags >> ((a - tok_a) & 63)) & ((2u << (n - 1)) - 1u);
     };
 
+    auto put = [&](window ow, frag f, unsigned off, int d) {     // elements d .. of the row at `off`; rows behind the window's end are not there
+        if (!ragged || d + V <= S.dv) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, f), ow, WHOLE || d < S.dv ? off + d * (unsigned)sizeof(T) : OUTSIDE, 0, 0);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (d + e < S.dv) {
+                    const T x = f[e];
+                    const unsigned at = off + (d + e) * (unsigned)sizeof(T);
+                    if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, x), ow, at, 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), ow, at, 0, 0);
+                }
+        }
+    };
+
     bool any_start = false;
     int pos = rev ? tok_e : tok_a, most = C;
     // (up to the next multiple of C: the first chunk of a reverse scan is the short one, and so is what follows tokens taken singly)
@@ -466,22 +481,8 @@ void seq_scan_kernel(const Args A) {
         }
         if constexpr (!STATE_ONLY) {
             const window ow = window_of(O + (long long)a * S.o_t, (unsigned)(n - 1) * o_t + row_v);
-            auto put = [&](frag f, unsigned off, int d) {   // elements d .. of a row
-                if (!ragged || d + V <= S.dv) {
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, f), ow, WHOLE || d < S.dv ? off + d * (unsigned)sizeof(T) : OUTSIDE, 0, 0);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (d + e < S.dv) {
-                            const T x = f[e];
-                            const unsigned at = off + (d + e) * (unsigned)sizeof(T);
-                            if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, x), ow, at, 0, 0);
-                            else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), ow, at, 0, 0);
-                        }
-                }
-            };
             if constexpr (PV <= 4 && NT == 1) {
-                put(Y::operand(o[0][0]), m * o_t, dv0 + g * V);
+                put(ow, Y::operand(o[0][0]), m * o_t, dv0 + g * V);
             } else {                                        // through LDS, so that neighbouring lanes store neighbouring pieces of a row
                 wave_sync();
 #pragma unroll
@@ -490,7 +491,7 @@ void seq_scan_kernel(const Args A) {
                     for (int jg = 0; jg < VS; ++jg) *(frag *)(ldsQ + Y::template at_rows<DVS>(16 * nt + m, KP * jg + g)) = Y::operand(o[jg][nt]);
                 wave_sync();
 #pragma unroll
-                for (int i = 0; i < NV; ++i) put(*(const frag *)(ldsQ + Y::template at_rows<DVS>(i * RV + rv, pv)), (unsigned)(i * RV + rv) * o_t, dvp);
+                for (int i = 0; i < NV; ++i) put(ow, *(const frag *)(ldsQ + Y::template at_rows<DVS>(i * RV + rv, pv)), (unsigned)(i * RV + rv) * o_t, dvp);
             }
         }
         // ---- the state behind the chunk
@@ -545,11 +546,10 @@ void seq_scan_kernel(const Args A) {
             A.carry[((long long)sc * A.a.B * A.a.H + bh) * nseg + seg] = any_start ? 0.f : power(lg, tok_e - tok_a);
     } else {
         // rows at and behind the length
-        for (int t = tok_e + rv; t < seg_e; t += RV) {
-            T *row = O + (long long)t * S.o_t;
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (dvp + e < S.dv) row[dvp + e] = (T)0.f;
+        const frag zero = __builtin_bit_cast(frag, u4{0u, 0u, 0u, 0u});
+        for (int t = tok_e; t < seg_e; t += RV) {
+            const int rows = seg_e - t < RV ? seg_e - t : RV;
+            put(window_of(O + (long long)t * S.o_t, (unsigned)(rows - 1) * o_t + row_v), zero, rv * o_t, dvp);
         }
         if ((rev ? seg == 0 : seg == nseg - 1) && S.s_out) {
             const gbytes_out p = shared_base_out(S.s_out + b * S.s_b + h * S.s_h);
@@ -616,7 +616,7 @@ int padded(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
 struct Plan { int dkp, dvs, n_sib, sib0[PVDER_SEQ_MAX_SCANS + 1]; };
 
 bool valid(const pvder_seq_attn *a) {
-    if (!a || a->n_scans < 1 || a->n_scans > PVDER_SEQ_MAX_SCANS || a->B < 0 || a->T < 0 || a->H < 1) return false;
+    if (!a || a->n_scans < 1 || a->n_scans > PVDER_SEQ_MAX_SCANS || a->B < 0 || a->T < 0 || a->T > PVDER_SEQ_MAX_TOKENS || a->H < 1) return false;
     if (a->dtype != PVDER_SEQ_F32 && a->dtype != PVDER_SEQ_BF16) return false;
     const int least = a->dtype == PVDER_SEQ_BF16 ? 8 : 4;  // 16 bytes: the kernels read rows in such pieces
     for (int i = 0; i < a->n_scans; ++i) {
@@ -673,8 +673,9 @@ template <typename T, int DKP, int DVS, bool WHOLE> int launch(const Args &A, co
     bool state = false;
     for (int i = 0; i < A.a.n_scans; ++i) state = state || A.a.scan[i].s_out != nullptr;
     if (A.a.segments > 1) {
-        seq_scan_kernel<T, DKP, DVS, WHOLE, true, MOST><<<grid, block, bytes, st>>>(A);
         const long long items = (long long)A.a.B * A.a.H * A.n_sib * (DKP * DVS / 4);
+        if (items / 256 >= 0x7fffffffll) return kEinval;
+        seq_scan_kernel<T, DKP, DVS, WHOLE, true, MOST><<<grid, block, bytes, st>>>(A);
         seq_join_kernel<T, DKP, DVS><<<dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st>>>(A);
     }
     if (state) seq_scan_kernel<T, DKP, DVS, WHOLE, false, MOST><<<grid, block, bytes, st>>>(A);
@@ -728,7 +729,7 @@ extern "C" int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream) {
         for (int i = 0; i < a->n_scans; ++i) {
             const pvder_seq_scan &s = a->scan[i];
             if (!s.q || !s.k || !s.v || !s.o) return kEinval;
-            if ((s.s_in || s.s_out) && (s.s_k < 0 || s.s_v < 0 || (s.dk * s.s_k + s.dv * s.s_v) >= (1ll << 29))) return kEinval;
+            if ((s.s_in || s.s_out) && (s.s_k < 0 || s.s_v < 0 || s.s_k >= (1ll << 29) || s.s_v >= (1ll << 29) || s.dk * s.s_k + s.dv * s.s_v >= (1ll << 29))) return kEinval;
             // (a row's end, where the window of a chunk ends, has to lie before the next row)
             if (s.q_t < s.dk || s.k_t < s.dk || s.v_t < s.dv || s.o_t < s.dv || s.q_t > most || s.k_t > most || s.v_t > most || s.o_t > most) return kEinval;
         }

@@ -14,7 +14,8 @@ extern "C" {
 #endif
 
 enum { PVDER_SEQ_F32 = 0, PVDER_SEQ_BF16 = 1 };
-enum { PVDER_SEQ_MAX_HEAD = 128, PVDER_SEQ_MAX_SCANS = 3, PVDER_SEQ_MAX_WIDTH = 8192, PVDER_SEQ_MAX_TOKEN_STRIDE = 1 << 26 };
+enum { PVDER_SEQ_MAX_HEAD = 128, PVDER_SEQ_MAX_SCANS = 3, PVDER_SEQ_MAX_WIDTH = 8192, PVDER_SEQ_MAX_TOKEN_STRIDE = 1 << 26,
+       PVDER_SEQ_MAX_TOKENS = 1 << 30 };
 
 /* One scan over the tokens of every (batch row b, head h): a state S of [dk, dv], fp32,
  *   forward :  S_t = g S_{t-1} + a_write k_t v_t^T,       o_t = a_read g S_{t-1}^T q_t + a_intra (q_t . k_t) v_t  (and so on within a chunk)

@@ -125,7 +125,7 @@ def test_c_entries_refuse_before_any_launch():
     from gym_PVDER_amd import _native
     _native.build_native()
     L = _native.sequence_lib()
-    for bad in (dict(dk=3), dict(dk=129), dict(dv=3), dict(dv=129), dict(dk=7, dtype=1), dict(dv=7, dtype=1), dict(B=-1), dict(T=-1), dict(H=0), dict(n=0), dict(n=4), dict(dtype=2)):
+    for bad in (dict(dk=3), dict(dk=129), dict(dv=3), dict(dv=129), dict(dk=7, dtype=1), dict(dv=7, dtype=1), dict(B=-1), dict(T=-1), dict(T=2 ** 30 + 1), dict(H=0), dict(n=0), dict(n=4), dict(dtype=2)):
         assert L.pvder_seq_attn_plan(_attn(**bad)) == _native.EINVAL, bad
         assert L.pvder_seq_attn_run(_attn(**bad), None) == _native.EINVAL, bad
     assert L.pvder_seq_attn_run(_attn(decay=0), None) == _native.EINVAL
