@@ -110,13 +110,23 @@ template <> struct Ty<float> {
 // LDS of a wave: a chunk's rows of Q, K and V
 template <typename T> constexpr int tile_bytes(int dkp, int dvs) { return (Ty<T>::size(dkp) + Ty<T>::size(dvs) + Ty<T>::size_rows(dkp > dvs ? dkp : dvs)) * (int)sizeof(T); }
 
+// Where the states that come into a scan's pieces lie: as the wave that made them held them, tile by tile, a strip of `side` tiles beside each
+// other after the other.  They may be of another scan, whose k is this one's v and whose v is its k: transposed then.
+struct States {
+    const float *at;                        // of the first (b, h, piece); `piece` floats further the next
+    long long piece;
+    int side_log2, strips, tiles;           // tiles of dk
+    bool transposed;
+};
+
 struct Args {
     pvder_seq_attn a;
     int seg_len, n_sib;                     // tokens of a piece; strips of one (b, h, piece), all scans together
     int sib0[PVDER_SEQ_MAX_SCANS + 1];      // first strip of each scan
     unsigned n_groups;                      // (b, h, piece) triples
-    long long per_sib;                      // workspace floats of one strip's state
+    long long per_sib;                      // state pass and join: workspace floats of one strip's state
     float *carry;                           // [scan][b][h][piece]: what a piece leaves of the state before it (0 behind a start)
+    States states[PVDER_SEQ_MAX_SCANS];     // main pass, several pieces
 };
 
 // Which (b, h, piece) and which of its scans a block is.  Blocks are dealt to the eight XCDs in turn: the scans of one triple read
@@ -188,12 +198,24 @@ void seq_scan_kernel(const Args A) {
                 }
     };
     const bool first = rev ? seg == nseg - 1 : seg == 0;
-    float *ws = A.a.workspace ? A.a.workspace + (((long long)grp * A.n_sib + sib) * A.per_sib) + lane * 4 : nullptr;
     if (!STATE_ONLY && nseg > 1) {
+        const States &W = A.states[sc];
+        const gbytes p = shared_base(W.at + grp * W.piece);
+        const int across = (16 * (m >> 2) + 4 * g) * 16 + 4 * (m & 3);      // element (m, 4 g) of a tile
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) s[i][j] = *(const f4 *)(ws + (i * NJ + j) * 256);
+            for (int j = 0; j < NJ; ++j) {
+                const int si = W.transposed ? strip * NJ + j : i, sj = W.transposed ? i : strip * NJ + j, of = sj >> W.side_log2;
+                const unsigned tile = (unsigned)((((of * W.tiles + si) << W.side_log2) + (sj & ((1 << W.side_log2) - 1))) * 1024);
+                s[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+                if (si < W.tiles && of < W.strips) {        // (what is padded further here than there is zero)
+                    if (!W.transposed) s[i][j] = *(const __attribute__((address_space(1))) f4 *)(p + tile + lane * 16);
+                    else
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[i][j][r] = *(const __attribute__((address_space(1))) float *)(p + tile + across + 16 * r);
+                }
+            }
     } else if (!STATE_ONLY && first && S.s_in) {
         const gbytes p = shared_base(S.s_in + b * S.s_b + h * S.s_h);
         state_elements([&](int i, int j, int r, bool is, unsigned at) {
@@ -538,6 +560,7 @@ void seq_scan_kernel(const Args A) {
     }
 
     if constexpr (STATE_ONLY) {
+        float *ws = A.a.workspace + ((long long)grp * A.n_sib + sib) * A.per_sib + lane * 4;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -615,6 +638,8 @@ int padded(int d) { return d <= 32 ? 32 : (d <= 64 ? 64 : 128); }
 // windows of 160 x 4 heads of 64, fp32, forward 35 us wide (256 waves), 20 us narrow (1024 waves).
 struct Plan { int dkp, dvs, n_sib, sib0[PVDER_SEQ_MAX_SCANS + 1]; };
 
+bool owns(const pvder_seq_scan &s) { return !s.kept && s.transpose_of == 0; }
+
 bool valid(const pvder_seq_attn *a) {
     if (!a || a->n_scans < 1 || a->n_scans > PVDER_SEQ_MAX_SCANS || a->B < 0 || a->T < 0 || a->T > PVDER_SEQ_MAX_TOKENS || a->H < 1) return false;
     if (a->dtype != PVDER_SEQ_F32 && a->dtype != PVDER_SEQ_BF16) return false;
@@ -622,16 +647,25 @@ bool valid(const pvder_seq_attn *a) {
     for (int i = 0; i < a->n_scans; ++i) {
         const pvder_seq_scan &s = a->scan[i];
         if (s.dk < least || s.dv < least || s.dk > PVDER_SEQ_MAX_HEAD || s.dv > PVDER_SEQ_MAX_HEAD) return false;
+        if (s.transpose_of < 0 || s.transpose_of > i || (s.transpose_of && s.kept) || ((uintptr_t)s.kept & 15)) return false;
+        if (s.transpose_of) {
+            const pvder_seq_scan &of = a->scan[s.transpose_of - 1];
+            if (!owns(of) || of.dk != s.dv || of.dv != s.dk) return false;
+        }
     }
     return true;
 }
 
-// The scans of `a` whose dk has the padded size dkp, as an argument of their own: scans of other sizes would be padded to the largest.
-int of_size(const pvder_seq_attn *a, int dkp, pvder_seq_attn &sub) {
+// The scans of `a` whose dk has the padded size dkp (`own`: that make their own states, too), as an argument of their own, and which they
+// are: scans of other sizes would be padded to the largest.
+int of_size(const pvder_seq_attn *a, int dkp, bool own, pvder_seq_attn &sub, int *which) {
     sub = *a;
     sub.n_scans = 0;
     for (int i = 0; i < a->n_scans; ++i)
-        if (padded(a->scan[i].dk) == dkp) sub.scan[sub.n_scans++] = a->scan[i];
+        if (padded(a->scan[i].dk) == dkp && (!own || owns(a->scan[i]))) {
+            which[sub.n_scans] = i;
+            sub.scan[sub.n_scans++] = a->scan[i];
+        }
     return sub.n_scans;
 }
 
@@ -664,66 +698,89 @@ int seg_len_of(const pvder_seq_attn *a) {
     return (per + c - 1) / c * c;
 }
 
-template <typename T, int DKP, int DVS, bool WHOLE> int launch(const Args &A, const Plan &P, hipStream_t st) {
+// The states of one scan of `a` among those that a plan lays into `at`
+States states_of(const float *at, const Plan &P, int scan, int dv, bool transposed) {
+    const long long strip = (long long)P.dkp * P.dvs;
+    const int side = P.dvs / 16;
+    return States{at + P.sib0[scan] * strip, P.n_sib * strip, side == 4 ? 2 : side - 1, (dv + P.dvs - 1) / P.dvs, P.dkp / 16, transposed};
+}
+
+// `states`: what each piece adds to the state and from that the states that come into the pieces; else the outputs
+template <typename T, int DKP, int DVS, bool WHOLE> int launch(const Args &A, bool states, hipStream_t st) {
     constexpr int MOST = sizeof(T) == 2 ? 3 : 1, LEAST = sizeof(T) == 2 ? 2 : 1;
     const long long blocks = (A.n_groups + 7ll) / 8 * 8 * A.n_sib;
     if (blocks > 0x7fffffffll) return kEinval;
     const dim3 grid((unsigned)blocks), block(64);
     const int bytes = tile_bytes<T>(DKP, DVS);
-    bool state = false;
-    for (int i = 0; i < A.a.n_scans; ++i) state = state || A.a.scan[i].s_out != nullptr;
-    if (A.a.segments > 1) {
+    if (states) {
         const long long items = (long long)A.a.B * A.a.H * A.n_sib * (DKP * DVS / 4);
         if (items / 256 >= 0x7fffffffll) return kEinval;
         seq_scan_kernel<T, DKP, DVS, WHOLE, true, MOST><<<grid, block, bytes, st>>>(A);
         seq_join_kernel<T, DKP, DVS><<<dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st>>>(A);
+    } else {
+        bool state = false;
+        for (int i = 0; i < A.a.n_scans; ++i) state = state || A.a.scan[i].s_out != nullptr;
+        if (state) seq_scan_kernel<T, DKP, DVS, WHOLE, false, MOST><<<grid, block, bytes, st>>>(A);
+        else seq_scan_kernel<T, DKP, DVS, WHOLE, false, LEAST><<<grid, block, bytes, st>>>(A);
     }
-    if (state) seq_scan_kernel<T, DKP, DVS, WHOLE, false, MOST><<<grid, block, bytes, st>>>(A);
-    else seq_scan_kernel<T, DKP, DVS, WHOLE, false, LEAST><<<grid, block, bytes, st>>>(A);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : -(int)e;
 }
 
-template <typename T, int DKP, int DVS> int fit(const Args &A, const Plan &P, hipStream_t st) {
+template <typename T, int DKP, int DVS> int fit(const Args &A, bool states, hipStream_t st) {
     bool whole = true;
     for (int i = 0; i < A.a.n_scans; ++i) whole = whole && A.a.scan[i].dk == DKP && A.a.scan[i].dv % DVS == 0;
-    return whole ? launch<T, DKP, DVS, true>(A, P, st) : launch<T, DKP, DVS, false>(A, P, st);
+    return whole ? launch<T, DKP, DVS, true>(A, states, st) : launch<T, DKP, DVS, false>(A, states, st);
 }
 
-template <typename T> int pick(const Args &A, const Plan &P, hipStream_t st) {
+template <typename T> int pick(const Args &A, const Plan &P, bool states, hipStream_t st) {
     constexpr int NARROW = sizeof(T) == 2 ? 32 : 16;
-    if (P.dkp == 32) return P.dvs == 64 ? fit<T, 32, 64>(A, P, st) : (P.dvs == 32 ? fit<T, 32, 32>(A, P, st) : fit<T, 32, NARROW>(A, P, st));
-    if (P.dkp == 64) return P.dvs == 64 ? fit<T, 64, 64>(A, P, st) : (P.dvs == 32 ? fit<T, 64, 32>(A, P, st) : fit<T, 64, NARROW>(A, P, st));
-    return P.dvs == 32 ? fit<T, 128, 32>(A, P, st) : fit<T, 128, NARROW>(A, P, st);
+    if (P.dkp == 32)
+        return P.dvs == 64 ? fit<T, 32, 64>(A, states, st) : (P.dvs == 32 ? fit<T, 32, 32>(A, states, st) : fit<T, 32, NARROW>(A, states, st));
+    if (P.dkp == 64)
+        return P.dvs == 64 ? fit<T, 64, 64>(A, states, st) : (P.dvs == 32 ? fit<T, 64, 32>(A, states, st) : fit<T, 64, NARROW>(A, states, st));
+    return P.dvs == 32 ? fit<T, 128, 32>(A, states, st) : fit<T, 128, NARROW>(A, states, st);
 }
 
 }  // namespace
 
 extern "C" int64_t pvder_seq_attn_plan(pvder_seq_attn *a) {
     if (!valid(a)) return kEinval;
+    pvder_seq_attn sub;
+    int which[PVDER_SEQ_MAX_SCANS];
+    bool given = false;
+    for (int i = 0; i < a->n_scans; ++i) given = given || a->scan[i].kept;
+    if (given && a->segments < 2) return kEinval;
     // Pieces of T side by side cost a second reading of K and V, a state of each piece in memory and two more launches: worth it where
     // the waves leave most of the card idle and the pieces make up for it.  Measured at heads of 64, bf16, one piece against the rule's:
     // 16 waves of 2048 tokens 82 us and 22 (32 pieces), 128 waves 84 and 35 (8); 512 waves 86 and 100 (4), 1024 waves of 512 61 and 86 (2).
-    pvder_seq_attn sub;
+    // With states that are there already pieces pay up to twice as many waves: forward and backward, 768 waves of 2048 tokens in the
+    // backward pass 262 us in one piece and 236 (fp32), 155 and 157 (bf16), 1152 waves of 1024 110 and 122.
     long long waves = 0;
     for (const int dkp : {32, 64, 128})
-        if (of_size(a, dkp, sub)) waves += (long long)a->B * a->H * plan_of(&sub, dkp).n_sib;
-    a->segments = 1;
-    if (waves >= 1 && waves <= 384 && a->T >= 384) {
-        const long long want = 2048 / waves, most = a->T / 64, n = want < most ? want : most;
-        if (n >= 4) a->segments = (int32_t)n;
+        if (of_size(a, dkp, false, sub, which)) waves += (long long)a->B * a->H * plan_of(&sub, dkp).n_sib;
+    if (given) {
+        if (waves > 768) a->segments = 1;
+    } else {
+        a->segments = 1;
+        if (waves >= 1 && waves <= 384 && a->T >= 384) {
+            const long long want = 2048 / waves, most = a->T / 64, n = want < most ? want : most;
+            if (n >= 4) a->segments = (int32_t)n;
+        }
     }
     if (a->segments == 1) return 0;
     int64_t floats = 0;
     for (const int dkp : {32, 64, 128})
-        if (of_size(a, dkp, sub)) floats += workspace_of(&sub, plan_of(&sub, dkp));
+        if (of_size(a, dkp, true, sub, which)) floats += workspace_of(&sub, plan_of(&sub, dkp));
     return floats;
 }
 
 extern "C" int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream) {
     if (!valid(a) || a->segments < 1 || !a->log_decay) return kEinval;
-    if (a->segments > 1 && (!a->workspace || ((uintptr_t)a->workspace & 15))) return kEinval;
     if ((long long)a->B * a->H * a->segments > 0x7fffffffll) return kEinval;
+    bool work_needed = false;
+    for (int i = 0; i < a->n_scans; ++i) work_needed = work_needed || (a->segments > 1 && owns(a->scan[i]));
+    if (work_needed && (!a->workspace || ((uintptr_t)a->workspace & 15))) return kEinval;
     if (a->B > 0 && a->T > 0) {
         const int64_t most = PVDER_SEQ_MAX_TOKEN_STRIDE / (a->dtype == PVDER_SEQ_BF16 ? 2 : 4);
         for (int i = 0; i < a->n_scans; ++i) {
@@ -732,25 +789,54 @@ extern "C" int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream) {
             if ((s.s_in || s.s_out) && (s.s_k < 0 || s.s_v < 0 || s.s_k >= (1ll << 29) || s.s_v >= (1ll << 29) || s.dk * s.s_k + s.dv * s.s_v >= (1ll << 29))) return kEinval;
             // (a row's end, where the window of a chunk ends, has to lie before the next row)
             if (s.q_t < s.dk || s.k_t < s.dk || s.v_t < s.dv || s.o_t < s.dv || s.q_t > most || s.k_t > most || s.v_t > most || s.o_t > most) return kEinval;
+            if (s.transpose_of) {
+                const pvder_seq_scan &of = a->scan[s.transpose_of - 1];
+                if (s.k != of.v || s.v != of.k || s.reverse != of.reverse || s.a_write != of.a_write) return kEinval;
+            }
         }
     }
     if (a->B == 0) return 0;
+    Args A = {};
+    const bool pieces = a->segments > 1 && a->T > 0;
+    States states[PVDER_SEQ_MAX_SCANS];
     float *work = a->workspace;
-    for (const int dkp : {32, 64, 128}) {
-        Args A;
-        if (!of_size(a, dkp, A.a)) continue;
-        if (A.a.T == 0) A.a.segments = 1;
-        const Plan P = plan_of(&A.a, dkp);
-        A.seg_len = A.a.T ? seg_len_of(&A.a) : 32;
-        A.n_sib = P.n_sib;
-        for (int i = 0; i <= PVDER_SEQ_MAX_SCANS; ++i) A.sib0[i] = P.sib0[i];
-        A.n_groups = (unsigned)((long long)a->B * a->H * A.a.segments);
-        A.per_sib = (long long)P.dkp * P.dvs;
-        A.a.workspace = work;
-        A.carry = A.a.segments > 1 ? work + (long long)A.n_groups * P.n_sib * A.per_sib : nullptr;
-        if (A.a.segments > 1) work += workspace_of(&A.a, P);
-        const int rc = a->dtype == PVDER_SEQ_BF16 ? pick<__bf16>(A, P, (hipStream_t)stream) : pick<float>(A, P, (hipStream_t)stream);
-        if (rc) return rc;
+    int which[PVDER_SEQ_MAX_SCANS];
+    for (const bool first : {true, false}) {               // the states of all pieces, then the outputs
+        if (first && !pieces) continue;
+        for (const int dkp : {32, 64, 128}) {
+            if (!of_size(a, dkp, first, A.a, which)) continue;
+            if (!pieces) A.a.segments = 1;
+            const Plan P = plan_of(&A.a, dkp);
+            A.seg_len = A.a.T ? seg_len_of(&A.a) : 32;
+            A.n_sib = P.n_sib;
+            for (int i = 0; i <= PVDER_SEQ_MAX_SCANS; ++i) A.sib0[i] = P.sib0[i];
+            A.n_groups = (unsigned)((long long)a->B * a->H * A.a.segments);
+            A.per_sib = (long long)P.dkp * P.dvs;
+            if (first) {
+                A.a.workspace = work;
+                A.carry = work + (long long)A.n_groups * P.n_sib * A.per_sib;
+                work += workspace_of(&A.a, P);
+                for (int i = 0; i < A.a.n_scans; ++i) states[which[i]] = states_of(A.a.workspace, P, i, A.a.scan[i].dv, false);
+            } else if (pieces) {
+                for (int i = 0; i < A.a.n_scans; ++i) {
+                    const pvder_seq_scan &s = A.a.scan[i];
+                    if (s.kept) {
+                        pvder_seq_attn was = *a;           // the run that left them
+                        was.n_scans = 1;
+                        was.scan[0].dk = s.dv;
+                        was.scan[0].dv = s.dk;
+                        A.states[i] = states_of(s.kept, plan_of(&was, padded(s.dv)), 0, s.dk, true);
+                    } else if (s.transpose_of) {
+                        A.states[i] = states[s.transpose_of - 1];
+                        A.states[i].transposed = true;
+                    } else {
+                        A.states[i] = states[which[i]];
+                    }
+                }
+            }
+            const int rc = a->dtype == PVDER_SEQ_BF16 ? pick<__bf16>(A, P, first, (hipStream_t)stream) : pick<float>(A, P, first, (hipStream_t)stream);
+            if (rc) return rc;
+        }
     }
     return 0;
 }

@@ -103,7 +103,7 @@ State state_strides(Maybe t, const Heads &d) {
 
 pvder_seq_scan scan_of(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &o, const void *s_in, void *s_out, const State &s, float a_read,
                        float a_write, float a_intra, bool reverse) {
-    pvder_seq_scan c;
+    pvder_seq_scan c = {};
     c.q = q.data_ptr(); c.k = k.data_ptr(); c.v = v.data_ptr(); c.o = o.data_ptr();
     const bool many = q.size(1) > 1;                       // (the stride of a single token says nothing: a row's length)
     c.q_b = q.stride(0); c.q_t = many ? q.stride(1) : q.size(3); c.q_h = q.stride(2);
@@ -117,8 +117,9 @@ pvder_seq_scan scan_of(const Tensor &q, const Tensor &k, const Tensor &v, const 
     return c;
 }
 
-// `a.scan` and `a.n_scans` are set; the rest comes from q's sizes and the options
-void run_scans(pvder_seq_attn &a, const Tensor &q, const Tensor &log_decay, Maybe starts, Maybe lengths) {
+// `a.scan` and `a.n_scans` are set (and a.segments, where they have states of an earlier run); the rest comes from q's sizes and the options.
+// Returns the workspace, undefined where T is one piece.
+Tensor run_scans(pvder_seq_attn &a, const Tensor &q, const Tensor &log_decay, Maybe starts, Maybe lengths) {
     a.log_decay = log_decay.data_ptr<float>();
     a.starts = (const uint8_t *)ptr(starts);
     a.starts_b = has(starts) ? starts->stride(0) : 0;
@@ -135,10 +136,17 @@ void run_scans(pvder_seq_attn &a, const Tensor &q, const Tensor &log_decay, Mayb
         a.workspace = work.data_ptr<float>();
     }
     checked(pvder_seq_attn_run(&a, stream_of(q)), "pvder_seq_attn_run");
+    return work;
 }
 
+// The states of the pieces of T as the forward pass left them, for the backward pass (at most 2048 strips of 16 KB)
+struct Kept {
+    Tensor states;
+    int32_t segments = 1;
+};
+
 std::tuple<Tensor, Tensor> attention_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &log_decay, Maybe initial, Maybe starts,
-                                             Maybe lengths, float scale, bool want_state) {
+                                             Maybe lengths, float scale, bool want_state, Kept *kept = nullptr) {
     const Heads d = {q.size(2), q.size(3), v.size(3)};
     const c10::DeviceGuard guard(q.device());
     Tensor out = at::empty({q.size(0), q.size(1), d.H, d.DV}, q.options()), final;
@@ -150,7 +158,8 @@ std::tuple<Tensor, Tensor> attention_forward(const Tensor &q, const Tensor &k, c
     pvder_seq_attn a;
     a.n_scans = 1;
     a.scan[0] = scan_of(q, k, v, out, ptr(in), want_state ? final.data_ptr() : nullptr, state_strides(in, d), scale, 1.f, scale, false);
-    run_scans(a, q, log_decay, starts, lengths);
+    const Tensor work = run_scans(a, q, log_decay, starts, lengths);
+    if (kept && work.defined()) *kept = {work, a.segments};
     return {out, final};
 }
 
@@ -177,9 +186,11 @@ struct DecayAttention : torch::autograd::Function<DecayAttention> {
                                                   const Tensor &log_decay, Maybe initial, Maybe starts, Maybe lengths, double scale, bool want_state) {
         ctx->set_materialize_grads(false);
         const Tensor none;
-        ctx->save_for_backward({q, k, v, log_decay, has(initial) ? *initial : none, has(starts) ? *starts : none, has(lengths) ? *lengths : none});
+        Kept kept;
+        auto [out, final] = attention_forward(q, k, v, log_decay, initial, starts, lengths, (float)scale, want_state, q.requires_grad() ? &kept : nullptr);
+        ctx->save_for_backward({q, k, v, log_decay, has(initial) ? *initial : none, has(starts) ? *starts : none, has(lengths) ? *lengths : none, kept.states});
         ctx->saved_data["scale"] = scale;
-        auto [out, final] = attention_forward(q, k, v, log_decay, initial, starts, lengths, (float)scale, want_state);
+        ctx->saved_data["segments"] = (int64_t)kept.segments;
         if (want_state) return {out, final};
         return {out};
     }
@@ -202,25 +213,30 @@ struct DecayAttention : torch::autograd::Function<DecayAttention> {
         const State plain = state_strides(optional<Tensor>(), d);
         pvder_seq_attn a;
         a.n_scans = 0;
+        a.segments = (int32_t)ctx->saved_data["segments"].toInt();
+        const bool need_v = ctx->needs_input_grad(2), need_s = has(initial) && ctx->needs_input_grad(4);
+        if (need_v || need_s) {
+            const Tensor dv = at::empty({q.size(0), q.size(1), d.H, d.DV}, q.options());
+            if (need_s) res[4] = at::empty({q.size(0), d.H, d.DK, d.DV}, log_decay.options());
+            a.scan[a.n_scans++] = scan_of(k, q, dout, dv, ds_in, need_s ? res[4].data_ptr() : nullptr, plain, 1.f, scale, scale, true);
+            res[2] = dv;
+        }
+        if (ctx->needs_input_grad(1)) {
+            res[1] = at::empty({q.size(0), q.size(1), d.H, d.DK}, q.options());
+            a.scan[a.n_scans] = scan_of(v, dout, q, res[1], ds_in, nullptr, {plain.b, plain.h, plain.v, plain.k}, 1.f, scale, scale, true);
+            a.scan[a.n_scans].transpose_of = a.n_scans;    // (dv's, if that is there)
+            ++a.n_scans;
+        }
         if (ctx->needs_input_grad(0)) {
             // dq_t = scale S_t do_t: the attention of do over (v, k), its state the transpose of S
             const State s = state_strides(initial, d);
             res[0] = at::empty({q.size(0), q.size(1), d.H, d.DK}, q.options());
-            a.scan[a.n_scans++] = scan_of(dout, v, k, res[0], ptr(initial), nullptr, {s.b, s.h, s.v, s.k}, scale, 1.f, scale, false);
-        }
-        if (ctx->needs_input_grad(1)) {
-            res[1] = at::empty({q.size(0), q.size(1), d.H, d.DK}, q.options());
-            a.scan[a.n_scans++] = scan_of(v, dout, q, res[1], ds_in, nullptr, {plain.b, plain.h, plain.v, plain.k}, 1.f, scale, scale, true);
-        }
-        const bool need_v = ctx->needs_input_grad(2), need_s = has(initial) && ctx->needs_input_grad(4);
-        Tensor dv;
-        if (need_v || need_s) {
-            dv = at::empty({q.size(0), q.size(1), d.H, d.DV}, q.options());
-            if (need_s) res[4] = at::empty({q.size(0), d.H, d.DK, d.DV}, log_decay.options());
-            a.scan[a.n_scans++] = scan_of(k, q, dout, dv, ds_in, need_s ? res[4].data_ptr() : nullptr, plain, 1.f, scale, scale, true);
-            if (need_v) res[2] = dv;
+            a.scan[a.n_scans] = scan_of(dout, v, k, res[0], ptr(initial), nullptr, {s.b, s.h, s.v, s.k}, scale, 1.f, scale, false);
+            if (saved[7].defined()) a.scan[a.n_scans].kept = saved[7].data_ptr<float>();
+            ++a.n_scans;
         }
         if (a.n_scans) run_scans(a, q, log_decay, starts, lengths);
+        if (!need_v) res[2] = Tensor();
         return res;
     }
 };

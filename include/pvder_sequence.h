@@ -29,8 +29,10 @@ typedef struct pvder_seq_scan {
     const float *s_in;              /* state that comes in, NULL: zeros; element (i, j) of (b, h) at b s_b + h s_h + i s_k + j s_v */
     float *s_out;                   /* state that goes out, NULL: not wanted; same strides */
     int64_t s_b, s_h, s_k, s_v;     /* s_k, s_v >= 0, dk s_k + dv s_v < 2^29 */
+    const float *kept;              /* NULL, or the workspace that an earlier run left: see below */
     float a_read, a_write, a_intra;
     int32_t dk, dv, reverse;        /* dk, dv: 16 bytes of elements (8 bf16, 4 fp32) .. PVDER_SEQ_MAX_HEAD */
+    int32_t transpose_of;           /* 0, or 1 + the number of an earlier scan of this call: see below */
 } pvder_seq_scan;
 
 typedef struct pvder_seq_attn {
@@ -43,8 +45,14 @@ typedef struct pvder_seq_attn {
     int32_t B, T, H, n_scans, dtype, segments;   /* segments: as pvder_seq_attn_plan() set it */
 } pvder_seq_attn;
 
-/* Sets a->segments, the pieces of T that run side by side, by B, T, H, n_scans, dtype and the scans' dk / dv alone (no pointer is
- * read), and returns the floats of workspace that they need (0: none); < 0: PVDER_EINVAL. */
+/* Sets a->segments, the pieces of T that run side by side, by B, T, H, n_scans, dtype and the scans' dk, dv, kept and transpose_of alone
+ * (no pointer is followed), and returns the floats of workspace that they need (0: none); < 0: PVDER_EINVAL.
+ *
+ * With several pieces a run first works out the state that comes into each, and leaves these states in the workspace.  A scan whose k is
+ * another's v and whose v is its k, in the same direction and with the same a_write, has that scan's states, transposed.  They are read
+ * instead of worked out again if the other is named: transpose_of in the same call, or, as kept, the workspace of an earlier run of that
+ * scan alone, with the same B, T, H, dtype, starts, lengths and (transposed) s_in.  Where a scan has kept, segments goes into the plan
+ * as the earlier run had it, and is left so, or set to 1: all of T in one piece then, and kept is not read. */
 int64_t pvder_seq_attn_plan(pvder_seq_attn *a);
 int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream);
 

@@ -89,6 +89,31 @@ def test_many_rows(ops, gpu_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1000, 2, 20, 64), (2, 520, 3, 64, 33), (1, 450, 1, 128, 48), (6, 390, 48, 8, 8)])
+def test_gradients_of_some_inputs_over_pieces(ops, gpu_device, shape, dtype):
+    """Long windows of few rows: every choice of the inputs that want a gradient, and the same graph walked twice.  (The last shape is cut
+    into pieces on the way forward only.)"""
+    B, T, H, DK, DV = shape
+    c = _case(*shape, dtype, gpu_device, True, True)
+    r, mag = _both(c, DK ** -0.5)
+    tol = ref.attention_bounds(dtype, T, DK, DV, r, mag)
+    r0, mag0 = _both({**c, "ds": None}, DK ** -0.5)
+    tol0 = ref.attention_bounds(dtype, T, DK, DV, r0, mag0)
+    leaf = {n: c[n].detach().requires_grad_() for n in ("q", "k", "v", "s0")}
+    outs = ops.decay_attention(leaf["q"], leaf["k"], leaf["v"], c["log_decay"], initial_state=leaf["s0"], starts=c["starts"], lengths=c["lengths"],
+                               output_final_state=True)
+    for choice in range(1, 16):
+        names = [n for i, n in enumerate(leaf) if choice >> i & 1]
+        first, again = (torch.autograd.grad(outs, [leaf[n] for n in names], [c["do"], c["ds"]], retain_graph=True) for _ in range(2))
+        assert all(torch.equal(x, y) for x, y in zip(first, again)), names
+        ref.check({"ds0" if n == "s0" else "d" + n: x for n, x in zip(names, first)}, r, tol, str(names))
+        own = {n: leaf[n].detach().requires_grad_(n in names) for n in leaf}
+        o = ops.decay_attention(own["q"], own["k"], own["v"], c["log_decay"], initial_state=own["s0"], starts=c["starts"], lengths=c["lengths"])
+        alone = torch.autograd.grad(o, [own[n] for n in names], c["do"])
+        ref.check({"ds0" if n == "s0" else "d" + n: x for n, x in zip(names, alone)}, r0, tol0, "alone %s" % names)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_layouts(ops, gpu_device, dtype):
     """Time-major tensors, one window seen by every row (stride 0), a head dimension that is not dense, states that are views."""
     B, T, H, DK, DV = 3, 40, 2, 16, 24

@@ -10,7 +10,7 @@ import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 # struct pvder_seq_scan, the rest of pvder_seq_attn, pvder_seq_step and pvder_seq_norm
-SCAN, ATTN_TAIL = struct.Struct("@4Q12q2Q4q3f3i"), struct.Struct("@4Q2q6i")
+SCAN, ATTN_TAIL = struct.Struct("@4Q12q2Q4qQ3f4i4x"), struct.Struct("@4Q2q6i")
 STEP, NORM = struct.Struct("@4Q8q3Q1q5i1f"), struct.Struct("@3Q3q6Q2Q2q5Q1q2i1f4x")
 HEADER = os.path.join(ROOT, "include", "pvder_sequence.h")
 
@@ -42,7 +42,7 @@ def test_packed_structs_match_the_header(tmp_path):
     subprocess.check_call(["gcc", "-I" + os.path.dirname(HEADER), str(src), "-o", str(exe)])
     got = [int(x) for x in subprocess.check_output([str(exe)]).split()]
     attn = 3 * SCAN.size + ATTN_TAIL.size
-    assert got == [SCAN.size, attn, STEP.size, NORM.size, attn - 4, struct.calcsize("@4Q12q2Q4q"), struct.calcsize("@4Q8q3Q1q"),
+    assert got == [SCAN.size, attn, STEP.size, NORM.size, attn - 4, struct.calcsize("@4Q12q2Q4qQ"), struct.calcsize("@4Q8q3Q1q"),
                    struct.calcsize("@3Q3q6Q2Q2q5Q"), so.MAX_HEAD, so.MAX_WIDTH]
 
 
@@ -115,7 +115,7 @@ def _attn(**tail):
     scan.update({k: tail.pop(k) for k in list(tail) if k in scan})
     row = max(scan["dk"], scan["dv"], 1) if tail.get("apart", True) else 0
     tail.pop("apart", None)
-    one = SCAN.pack(*([64] * 4), *([0, row, 0] * 4), 0, 0, *([0] * 4), 1.0, 1.0, 1.0, scan["dk"], scan["dv"], 0)
+    one = SCAN.pack(*([64] * 4), *([0, row, 0] * 4), 0, 0, *([0] * 4), tail.pop("kept", 0), 1.0, 1.0, 1.0, scan["dk"], scan["dv"], 0, tail.pop("of", 0))
     d = dict(decay=64, work=0, B=1, T=8, H=1, n=1, dtype=0, segments=1)
     d.update(tail)
     return ctypes.create_string_buffer(one * 3 + ATTN_TAIL.pack(d["decay"], 0, 0, d["work"], 0, 0, d["B"], d["T"], d["H"], d["n"], d["dtype"], d["segments"]))
@@ -133,6 +133,13 @@ def test_c_entries_refuse_before_any_launch():
     assert L.pvder_seq_attn_run(_attn(segments=0), None) == _native.EINVAL
     assert L.pvder_seq_attn_run(_attn(segments=2), None) == _native.EINVAL          # no workspace
     assert L.pvder_seq_attn_run(_attn(segments=2, work=68), None) == _native.EINVAL  # a workspace that is not aligned
+    for bad in (dict(of=1), dict(of=-1), dict(of=4), dict(kept=68), dict(kept=64, of=1)):    # states of a scan that is not there, or not one's own
+        assert L.pvder_seq_attn_run(_attn(n=3, **bad), None) == _native.EINVAL, bad
+        assert L.pvder_seq_attn_plan(_attn(n=3, segments=4, **bad)) == _native.EINVAL, bad
+    assert L.pvder_seq_attn_plan(_attn(kept=64)) == _native.EINVAL                       # of a run in one piece
+    some, many = _attn(kept=64, segments=4), _attn(B=200, H=4, T=512, kept=64, segments=4)
+    assert L.pvder_seq_attn_plan(some) == 0 and L.pvder_seq_attn_plan(many) == 0
+    assert [struct.unpack_from("@i", a, len(a.raw) - 5)[0] for a in (some, many)] == [4, 1]
     assert L.pvder_seq_attn_run(None, None) == _native.EINVAL
     assert L.pvder_seq_attn_plan(_attn()) == 0
     assert L.pvder_seq_attn_run(_attn(B=0), None) == 0
