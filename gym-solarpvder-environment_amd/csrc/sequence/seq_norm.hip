@@ -14,7 +14,6 @@ namespace {
 
 using namespace pvder_seq;
 
-
 // threads of a block: 256 where a wave holds whole rows, else one row's
 constexpr int block_of(int tpr) { return tpr > 64 ? tpr : 256; }
 
@@ -143,12 +142,13 @@ template <typename T, int TPR, int NV, bool EVEN> __global__ __launch_bounds__(b
     }
 }
 
-template <typename T, int TPR, int NV, bool EVEN> __global__ __launch_bounds__(block_of(TPR)) void seq_norm_backward_kernel(const pvder_seq_norm a) {
+template <typename T, int TPR, int NV, bool EVEN> __global__ __launch_bounds__(block_of(TPR)) __attribute__((amdgpu_waves_per_eu(TPR == 512 && Row<T, NV>::E == 8 ? 4 : 1)))
+void seq_norm_backward_kernel(const pvder_seq_norm a) {
     constexpr int BLOCK = block_of(TPR), RPB = BLOCK / TPR, V = Vec<T>::N, E = Row<T, NV>::E;
     typedef typename Vec<T>::type vec;
-    // Rows of more than 4096 (16 elements a lane): h' and the sigmoid are taken a second time and the weights come from L2 row by row;
-    // held in registers they would not fit
-    constexpr bool LEAN = E > 8;
+    // TWICE, rows of over 2048: h' and the sigmoid are taken a second time instead of held, so that two blocks of eight waves find room on a
+    // CU: 16384 x 4096, bf16, 442 us -> 303.  LEAN, over 4096 (16 elements a lane): the weights come from L2 a vector at a time, too.
+    constexpr bool LEAN = E > 8, TWICE = TPR == 512;
     __shared__ float lds[TPR > 64 ? TPR / 64 : 1];
     __shared__ float sums[RPB > 1 ? RPB * TPR * E : 1];
     const int t = threadIdx.x % TPR, D = a.width, grp = threadIdx.x / TPR;
@@ -180,14 +180,14 @@ template <typename T, int TPR, int NV, bool EVEN> __global__ __launch_bounds__(b
         row(dx, a.dx, a.dx_r);
         row(dh, a.dh, a.dh_r);
         const float ry = a.stats[2 * r], rh = a.stats[2 * r + 1];
-        Row<T, LEAN ? 1 : NV> hn, sg, sc;
+        Row<T, TWICE ? 1 : NV> hn, sg, sc;
         Row<T, NV> dn;
         auto branch = [&](int i, int k) {                   // element k of vector i of h', the sigmoid and its derivative
-            const int e = LEAN ? k : i * V + k;
+            const int e = TWICE ? k : i * V + k, p = LEAN ? k : i * V + k;
             sg.e[e] = 1.f;
             sc.e[e] = 0.f;
             if (a.gate) sigmoids((float)z[i][k], sg.e[e], sc.e[e]);
-            hn.e[e] = __builtin_fmaf(scale.e[e], (float)y[i][k] * ry * post.e[e] * sg.e[e], (float)h[i][k]);
+            hn.e[e] = __builtin_fmaf(scale.e[p], (float)y[i][k] * ry * post.e[p] * sg.e[e], (float)h[i][k]);
         };
         float s = 0.f;
 #pragma unroll
@@ -195,23 +195,27 @@ template <typename T, int TPR, int NV, bool EVEN> __global__ __launch_bounds__(b
             if constexpr (LEAN) weights(i);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                const int e = LEAN ? k : i * V + k;
+                const int e = TWICE ? k : i * V + k, p = LEAN ? k : i * V + k;
                 branch(i, k);
-                s = __builtin_fmaf((float)dx[i][k] * pre.e[e], hn.e[e], s);
+                s = __builtin_fmaf((float)dx[i][k] * pre.e[p], hn.e[e], s);
             }
             if constexpr (LEAN) apart();
         }
         const float A = row_sum<TPR>(s, lds) * inv * rh * rh;
+        if constexpr (TWICE) {                             // (so that the compiler does not hold them after all)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(z[i]), "+v"(y[i]), "+v"(h[i]));
+        }
         s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if constexpr (LEAN) weights(i);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                const int e = LEAN ? k : i * V + k, x0 = i * V + k;
-                if constexpr (LEAN) branch(i, k);
-                const float x = (float)dx[i][k], n0 = (float)y[i][k] * ry, n = n0 * post.e[e];
-                const float d = __builtin_fmaf(rh, x * pre.e[e] - hn.e[e] * A, (float)dh[i][k]), du = d * scale.e[e];
+                const int e = TWICE ? k : i * V + k, p = LEAN ? k : i * V + k, x0 = i * V + k;
+                if constexpr (TWICE) branch(i, k);
+                const float x = (float)dx[i][k], n0 = (float)y[i][k] * ry, n = n0 * post.e[p];
+                const float d = __builtin_fmaf(rh, x * pre.e[p] - hn.e[e] * A, (float)dh[i][k]), du = d * scale.e[p];
                 if (on) {                                  // (a row past the end stands in for the block's first)
                     gpre.e[x0] = __builtin_fmaf(x * hn.e[e], rh, gpre.e[x0]);
                     gscale.e[x0] = __builtin_fmaf(d, n * sg.e[e], gscale.e[x0]);
@@ -219,7 +223,7 @@ template <typename T, int TPR, int NV, bool EVEN> __global__ __launch_bounds__(b
                 }
                 z[i][k] = (T)(sc.e[e] * du * n);
                 dh[i][k] = (T)d;
-                dn.e[x0] = du * sg.e[e] * post.e[e];
+                dn.e[x0] = du * sg.e[e] * post.e[p];
                 s = __builtin_fmaf(dn.e[x0], (float)y[i][k], s);
             }
             if constexpr (LEAN) apart();
@@ -296,11 +300,14 @@ long long blocks_of(long long rows, int tpr, int waves) {
     const long long turns = (need + most - 1) / most;
     return (need + turns - 1) / turns;
 }
-constexpr int kForwardWaves = 24, kBackwardWaves = 12;
+// Waves on a CU: a whole number of blocks that it holds at once.  (Backward, 512 lanes to a row: 12 waves are one and a half blocks,
+// 16384 x 5000, fp32, 1172 us, 16 waves 946.)
+constexpr int kForwardWaves = 24;
+constexpr int backward_waves(int tpr) { return tpr == 512 ? 16 : 12; }
 
 template <typename T, int TPR, int NV, bool EVEN> void start(const pvder_seq_norm &a, bool back, hipStream_t st) {
     constexpr int BLOCK = block_of(TPR);
-    const unsigned blocks = (unsigned)blocks_of(a.rows, TPR, back ? kBackwardWaves : kForwardWaves);
+    const unsigned blocks = (unsigned)blocks_of(a.rows, TPR, back ? backward_waves(TPR) : kForwardWaves);
     if (back) {
         seq_norm_backward_kernel<T, TPR, NV, EVEN><<<dim3(blocks), dim3(BLOCK), 0, st>>>(a);
         if (a.dparam && blocks > 1)
@@ -341,7 +348,7 @@ bool ok(const pvder_seq_norm *a) {
 extern "C" int64_t pvder_seq_norm_workspace(const pvder_seq_norm *a) {
     if (!ok(a)) return kEinval;
     if (!a->dparam || a->rows == 0) return 0;
-    const long long blocks = blocks_of(a->rows, lanes_of(a->width), kBackwardWaves);
+    const long long blocks = blocks_of(a->rows, lanes_of(a->width), backward_waves(lanes_of(a->width)));
     return blocks > 1 ? blocks * 3 * a->width : 0;
 }
 

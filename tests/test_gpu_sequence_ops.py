@@ -307,7 +307,7 @@ def _norm_run(ops, c, eps=1e-6, which=("dh", "dx")):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("gate,scale", [(True, True), (False, False), (True, False), (False, True)])
-@pytest.mark.parametrize("R,D", [(1, 1), (1, 128), (3, 3), (5, 16), (300, 17), (1025, 100), (64, 128), (7, 513), (33, 1024), (2100, 64), (10, 2048),
+@pytest.mark.parametrize("R,D", [(1, 1), (600, 5000), (1100, 2500), (1, 128), (3, 3), (5, 16), (300, 17), (1025, 100), (64, 128), (7, 513), (33, 1024), (2100, 64), (10, 2048),
                                  (3, 4100), (5, 8192), (2, 8191)])
 def test_norm(ops, gpu_device, R, D, gate, scale, dtype):
     c = _norm_case(R, D, dtype, gpu_device, gate, scale)
