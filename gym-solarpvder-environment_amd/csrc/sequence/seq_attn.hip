@@ -7,10 +7,23 @@
 //   S   = g^C S + K^T (w V)              [dk x strip]  w_y = g^(C - 1 - y)
 // All three are computed transposed, so that the accumulators of one product already lie as the operand of the next: the row
 // that a lane's accumulator r of tile t stands for is chosen (`tile_row`) so that the lane holds exactly the contraction slots
-// it has to supply.  P and S never pass through LDS; K and V do, once, to be read back by columns.
+// it has to supply.  P and S stay in registers.  Q, K and V come in whole lines, one chunk ahead, and pass through LDS, to be read
+// by rows (Q, K) and by columns (K, V); the output goes through the place of Q, to leave in whole lines too.
+//
+// Long T with few heads is cut into pieces that run side by side, in three launches: what each piece adds to the state
+// (`STATE_ONLY`), the states that come into the pieces (seq_join_kernel), and the outputs.  The three gradients are scans too; of
+// their piece states the backward pass works out one, that of dv: dk's is its transpose, dq's the transpose of the forward pass's.
 //
 // Bound: bytes.  A token of a head costs (2 dk + 2 dv) elements and 4 dk dv + 2 C (dk + dv) operations: with bf16, dk = dv = 64
-// and C = 32 that is 48 operations per byte, where the card turns over at about 240.
+// and C = 32 that is 48 operations per byte, where the card turns over at about 240.  fp32 has C = 16 and matrix instructions of an
+// eighth of the rate: 20 operations per byte of the 30 at which it turns over.
+//
+// Measured, time of the kernels and share of 5.2 TB/s for each tensor once: forward 128 windows of 2048 tokens x 16 heads of 64,
+// bf16, 489 us, 85 %; 1024 tokens, fp32, 478 us, 86 %; heads of 128, bf16, 64 x 1024 x 16, 376 us, 55 % (the state fills the
+// registers and each strip of 32 columns reads Q and K again); heads of 32, 512 x 1024 x 8, 259 us, 80 %.  In pieces: one stream of
+// 16384 tokens x 8 heads of 128, bf16, 94 us, 28 % (states 26, join 18, outputs 50); forward and backward, 4 x 4096 x 16 heads of 64,
+// bf16, 172 us, 30 %.  Windows of 160 x 4 heads of 64, 64 of them, fp32, forward and backward, 61 us, 20 % (latency: ten chunks, one
+// behind the other).
 #include "seq_common.hpp"
 
 namespace {
@@ -124,17 +137,20 @@ struct Args {
     int seg_len, n_sib;                     // tokens of a piece; strips of one (b, h, piece), all scans together
     int sib0[PVDER_SEQ_MAX_SCANS + 1];      // first strip of each scan
     unsigned n_groups;                      // (b, h, piece) triples
+    unsigned together_log2;                 // how many of them on end belong to one XCD
     long long per_sib;                      // state pass and join: workspace floats of one strip's state
     float *carry;                           // [scan][b][h][piece]: what a piece leaves of the state before it (0 behind a start)
     States states[PVDER_SEQ_MAX_SCANS];     // main pass, several pieces
 };
 
-// Which (b, h, piece) and which of its scans a block is.  Blocks are dealt to the eight XCDs in turn: the scans of one triple read
-// the same tensors, so they get block numbers that are 8 apart and share one L2.
-__device__ __forceinline__ bool whose(const Args &A, unsigned &grp, int &sc) {
+// Which (b, h, piece) a block is of, and which of its strips, all scans together.  Blocks are dealt to the eight XCDs in turn: the strips
+// of one triple read the same tensors, so they get block numbers that are 8 apart and share one L2.  So do four triples on end where that
+// pays (`fours`).
+__device__ __forceinline__ bool whose(const Args &A, unsigned &grp, int &sib) {
     const unsigned row = (blockIdx.x >> 3) / (unsigned)A.n_sib;
-    sc = (int)((blockIdx.x >> 3) - row * (unsigned)A.n_sib);
-    grp = row * 8 + (blockIdx.x & 7);
+    sib = (int)((blockIdx.x >> 3) - row * (unsigned)A.n_sib);
+    const unsigned t = (1u << A.together_log2) - 1u;
+    grp = ((((row >> A.together_log2) * 8 + (blockIdx.x & 7)) << A.together_log2) + (row & t));
     return grp < A.n_groups;
 }
 
@@ -151,10 +167,8 @@ void seq_scan_kernel(const Args A) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
     unsigned grp;
-    int sc;
-    if (!whose(A, grp, sc)) return;
-    const int sib = sc;
-    sc = 0;
+    int sib, sc = 0;
+    if (!whose(A, grp, sib)) return;
     while (sc + 1 < A.a.n_scans && sib >= A.sib0[sc + 1]) ++sc;
     const pvder_seq_scan &S = A.a.scan[sc];
     const int strip = sib - A.sib0[sc], dv0 = strip * DVS;
@@ -583,7 +597,9 @@ void seq_scan_kernel(const Args A) {
     }
 }
 
-// The states that come into the pieces, from what each piece adds: s_(i+1) = carry_i s_i + u_i, written over u_i as s_i.
+// The states that come into the pieces, from what each piece adds: s_(i+1) = carry_i s_i + u_i, written over u_i as s_i.  A lane takes four
+// elements through all pieces.  Bound: the states, read and written once (64 pieces of 8 heads of 128: 67 MB, 18 us, 3.8 TB/s; 16 or 32
+// loads in flight instead of 8 take the same).
 template <typename T, int DKP, int DVS> __global__ __launch_bounds__(256) void seq_join_kernel(const Args A) {
     typedef Ty<T> Y;
     constexpr int Q = DKP * DVS / 4, TT = Y::TT, NJ = DVS / 16;
@@ -688,6 +704,15 @@ Plan plan_of(const pvder_seq_attn *a, int dkp) {
     return P;
 }
 
+// Whether four (b, h, piece) on end go to one XCD: where there are enough to go round, and rows of less than a line share theirs with the
+// next head's (512 x 1024 x 8 heads of 32, bf16: 290 us one by one, 259 by fours, 256 by eights) or heads are of 128 (64 x 1024 x 16: 393,
+// 376, 378).  Else it is no gain: 128 x 2048 x 16 heads of 64 486, 491, 504; 64 windows of 160 x 4 heads of 64, fp32, 61.5, 63, 63.
+bool fours(const pvder_seq_attn &a, unsigned n_groups, int dkp) {
+    bool shared = dkp == 128;
+    for (int i = 0; i < a.n_scans; ++i) shared = shared || (a.scan[i].dk < a.scan[i].dv ? a.scan[i].dk : a.scan[i].dv) * (a.dtype == PVDER_SEQ_BF16 ? 2 : 4) < 128;
+    return shared && n_groups >= 256;
+}
+
 int64_t workspace_of(const pvder_seq_attn *a, const Plan &P) {
     const int64_t bhs = (int64_t)a->B * a->H * a->segments;
     return (bhs * P.n_sib * P.dkp * P.dvs + bhs * a->n_scans + 3) / 4 * 4;      // (whole 16 bytes: the next size's begins there)
@@ -708,7 +733,7 @@ States states_of(const float *at, const Plan &P, int scan, int dv, bool transpos
 // `states`: what each piece adds to the state and from that the states that come into the pieces; else the outputs
 template <typename T, int DKP, int DVS, bool WHOLE> int launch(const Args &A, bool states, hipStream_t st) {
     constexpr int MOST = sizeof(T) == 2 ? 3 : 1, LEAST = sizeof(T) == 2 ? 2 : 1;
-    const long long blocks = (A.n_groups + 7ll) / 8 * 8 * A.n_sib;
+    const long long deal = 8ll << A.together_log2, blocks = (A.n_groups + deal - 1) / deal * deal * A.n_sib;
     if (blocks > 0x7fffffffll) return kEinval;
     const dim3 grid((unsigned)blocks), block(64);
     const int bytes = tile_bytes<T>(DKP, DVS);
@@ -811,6 +836,7 @@ extern "C" int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream) {
             A.n_sib = P.n_sib;
             for (int i = 0; i <= PVDER_SEQ_MAX_SCANS; ++i) A.sib0[i] = P.sib0[i];
             A.n_groups = (unsigned)((long long)a->B * a->H * A.a.segments);
+            A.together_log2 = fours(A.a, A.n_groups, dkp) ? 2 : 0;
             A.per_sib = (long long)P.dkp * P.dvs;
             if (first) {
                 A.a.workspace = work;

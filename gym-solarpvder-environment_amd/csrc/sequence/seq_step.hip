@@ -4,6 +4,8 @@
 //
 // Bound: the state, read and written once: 8 dk dv bytes of 8 dk dv + (2 dk + 2 dv) elements.  A lane holds 16 bytes of a row of
 // S and walks down the rows; the lanes beside it hold the rest of the row, so that a wave reads whole rows.
+// Measured: 65 536 envs x 4 heads of 32 x 32, fp32, 404 us, 2.28 GB at 5.65 TB/s; 1001 envs x 3 heads of 48 x 80, bf16, 17 us, 93 MB at
+// 5.4 TB/s; one env 3.7 us, which is what a launch takes.
 #include "seq_common.hpp"
 
 namespace {

@@ -17,10 +17,11 @@ enum { PVDER_SEQ_F32 = 0, PVDER_SEQ_BF16 = 1 };
 enum { PVDER_SEQ_MAX_HEAD = 128, PVDER_SEQ_MAX_SCANS = 3, PVDER_SEQ_MAX_WIDTH = 8192, PVDER_SEQ_MAX_TOKEN_STRIDE = 1 << 26,
        PVDER_SEQ_MAX_TOKENS = 1 << 30 };
 
-/* One scan over the tokens of every (batch row b, head h): a state S of [dk, dv], fp32,
- *   forward :  S_t = g S_{t-1} + a_write k_t v_t^T,       o_t = a_read g S_{t-1}^T q_t + a_intra (q_t . k_t) v_t  (and so on within a chunk)
- *   reverse :  the same from the last token to the first
- * With a_intra = a_read * a_write this is o_t = a_read S_t^T q_t.  The three gradients of an attention are scans of its inputs
+/* One scan over the tokens of every (batch row b, head h): a state S of [dk, dv], fp32.
+ *   forward :  R_t = g S_(t-1);  o_t = a_read R_t^T q_t + a_intra (q_t . k_t) v_t;  S_t = R_t + a_write k_t v_t^T
+ *   reverse :  S is what the later tokens left, the weight g comes behind the token and not before it:
+ *              o_t = a_read S_(t+1)^T q_t + a_intra (q_t . k_t) v_t;  S_t = g (S_(t+1) + a_write k_t v_t^T)
+ * With a_intra = a_read * a_write the forward form is o_t = a_read S_t^T q_t.  The three gradients of an attention are scans of its inputs
  * in other places:  dq = scan(do, v, k),  dk = reverse scan(v, do, q),  dv = reverse scan(k, q, do). */
 typedef struct pvder_seq_scan {
     const void *q, *k, *v;          /* [B, T, H, dk], [B, T, H, dk], [B, T, H, dv] */
