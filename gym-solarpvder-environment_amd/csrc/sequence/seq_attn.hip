@@ -708,7 +708,7 @@ Plan plan_of(const pvder_seq_attn *a, int dkp) {
 // next head's (512 x 1024 x 8 heads of 32, bf16: 290 us one by one, 259 by fours, 256 by eights) or heads are of 128 (64 x 1024 x 16: 393,
 // 376, 378).  Else it is no gain: 128 x 2048 x 16 heads of 64 486, 491, 504; 64 windows of 160 x 4 heads of 64, fp32, 61.5, 63, 63.
 bool fours(const pvder_seq_attn &a, unsigned n_groups, int dkp) {
-    bool shared = dkp == 128;
+    bool shared = dkp == 128 && a.segments == 1;
     for (int i = 0; i < a.n_scans; ++i) shared = shared || (a.scan[i].dk < a.scan[i].dv ? a.scan[i].dk : a.scan[i].dv) * (a.dtype == PVDER_SEQ_BF16 ? 2 : 4) < 128;
     return shared && n_groups >= 256;
 }
