@@ -260,6 +260,7 @@ py::object decay_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_,
     }
     const float scale = scale_of(scale_, d.DK);
     on_gpu(q_, "q");
+    const c10::DeviceGuard guard(q_.device());
     const int64_t least = 16 / (int64_t)q_.element_size();
     if (d.DK < least || d.DV < least) {
         // heads of less than 16 bytes: with zeros behind them, and without them again
@@ -271,7 +272,7 @@ py::object decay_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_,
         auto cut = [&](const py::handle &o) { return o.cast<Tensor>().narrow(-1, 0, d.DV); };
         if (!want_state) return py::cast(cut(r));
         const py::tuple both = r.cast<py::tuple>();
-        return py::make_tuple(cut(both[0]), cut(both[1]).narrow(2, 0, d.DK));
+        return py::make_tuple(cut(both[0]), cut(both[1]).narrow(2, 0, d.DK).contiguous());      // (as the step form wants it)
     }
     const Tensor q = tokens(q_), k = tokens(k_), v = tokens(v_);
     const optional<Tensor> initial = has(initial_) ? optional<Tensor>(dense(*initial_)) : optional<Tensor>();
@@ -431,6 +432,7 @@ std::tuple<Tensor, Tensor> gated_residual_norm(const Tensor &h, const Tensor &y,
     if (has(scale)) weight(*scale, "scale");
     NEED(std::isfinite((float)eps) && eps >= 0.0, "eps must be a finite number >= 0");
     on_gpu(h, "residual");
+    const c10::DeviceGuard guard(h.device());
     if (at::GradMode::is_enabled() && (wants_grad(h) || wants_grad(y) || wants_grad(post) || wants_grad(pre) || wants_grad(gate) || wants_grad(scale))) {
         if (capturing()) {
             const Tensor *all[] = {&h, &y, &post, &pre, has(gate) ? &*gate : nullptr, has(scale) ? &*scale : nullptr};

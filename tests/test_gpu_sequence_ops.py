@@ -472,6 +472,43 @@ def test_a_long_cache_of_offsets(ops, gpu_device):
     assert torch.equal(ops.decay_attention(c["q"][:1, :5], c["k"][:1, :5], tokens, c["log_decay"]), want[:1, :5])
 
 
+def test_many_rows_of_offsets(ops, gpu_device):
+    """Norm rows and states over 2^31 elements into their tensors: the last of them as if they were alone."""
+    R, D = 270_000, 8192
+    y = torch.empty(R, D, dtype=torch.bfloat16, device=gpu_device)
+    y[:-300] = 1.0
+    y[-300:] = torch.randn(300, D, generator=_gen(5)).to(torch.bfloat16).to(gpu_device)
+    post, pre = torch.rand(D, generator=_gen(6)).to(gpu_device), torch.rand(D, generator=_gen(7)).to(gpu_device)
+    h, x = ops.gated_residual_norm(y, y, post, pre, gate=y)
+    h1, x1 = ops.gated_residual_norm(y[-300:], y[-300:], post, pre, gate=y[-300:])
+    assert torch.equal(h[-300:], h1) and torch.equal(x[-300:], x1)
+    del h, x
+    leaf, last = y.detach().requires_grad_(), y[-300:].detach().requires_grad_()
+    g = torch.autograd.grad(ops.gated_residual_norm(leaf, leaf, post, pre), [leaf], [y, y])[0]
+    assert torch.equal(g[-300:], torch.autograd.grad(ops.gated_residual_norm(last, last, post, pre), [last], [y[-300:], y[-300:]])[0])
+    del y, leaf, last, g
+    N, H, K = 140_000, 1, 128
+    state = torch.zeros(N, H, K, K, device=gpu_device)
+    q, k, v = (torch.randn(N, H, K, generator=_gen(s)).to(gpu_device) for s in (1, 2, 3))
+    state[-9:] = torch.randn(9, H, K, K, generator=_gen(4)).to(gpu_device)
+    few, decay = state[-9:].clone(), torch.full((H,), -0.1, device=gpu_device)
+    out = ops.decay_attention_step(q, k, v, decay, state)
+    assert torch.equal(out[-9:], ops.decay_attention_step(q[-9:], k[-9:], v[-9:], decay, few)) and torch.equal(state[-9:], few)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_small_heads_go_on_in_steps(ops, gpu_device, dtype):
+    """Heads of less than 16 bytes: the window's state is one that the step form takes."""
+    c = _case(2, 9, 2, 3, 1, dtype, gpu_device, False, True)
+    whole, end = ops.decay_attention(c["q"], c["k"], c["v"], c["log_decay"], initial_state=c["s0"], output_final_state=True)
+    out, state = ops.decay_attention(c["q"][:, :8], c["k"][:, :8], c["v"][:, :8], c["log_decay"], initial_state=c["s0"], output_final_state=True)
+    last = ops.decay_attention_step(c["q"][:, 8], c["k"][:, 8], c["v"][:, 8], c["log_decay"], state)
+    r, mag = _both({**c, "do": torch.zeros_like(c["do"]), "ds": torch.zeros_like(c["ds"])}, 3 ** -0.5)
+    tol = ref.attention_bounds(dtype, 9, 3, 1, r, mag)
+    ref.check({"out": torch.cat([out, last[:, None]], 1), "state": state}, {"out": r["out"], "state": r["state"]}, tol)
+    ref.check({"out": whole, "state": end}, {"out": r["out"], "state": r["state"]}, tol)
+
+
 def test_a_second_derivative_is_refused(ops, gpu_device):
     c, nc = _case(1, 9, 1, 8, 8, torch.float32, gpu_device), _norm_case(4, 8, torch.float32, gpu_device)
     q = c["q"].detach().requires_grad_()
