@@ -19,7 +19,7 @@
 // eighth of the rate: 20 operations per byte of the 30 at which it turns over.
 //
 // Measured, time of the kernels and share of 5.2 TB/s for each tensor once: forward 128 windows of 2048 tokens x 16 heads of 64,
-// bf16, 489 us, 85 %; 1024 tokens, fp32, 478 us, 86 %; heads of 128, bf16, 64 x 1024 x 16, 376 us, 55 % (the state fills the
+// bf16, 489 us, 85 %; 1024 tokens, fp32, 478 us, 86 %; heads of 128, bf16, 64 x 1024 x 16, 308 us, 67 % (the state fills the
 // registers and each strip of 32 columns reads Q and K again); heads of 32, 512 x 1024 x 8, 259 us, 80 %.  In pieces: one stream of
 // 16384 tokens x 8 heads of 128, bf16, 94 us, 28 % (states 26, join 18, outputs 50); forward and backward, 4 x 4096 x 16 heads of 64,
 // bf16, 172 us, 30 %.  Windows of 160 x 4 heads of 64, 64 of them, fp32, forward and backward, 61 us, 20 % (latency: ten chunks, one
@@ -164,6 +164,10 @@ void seq_scan_kernel(const Args A) {
     typedef typename Y::frag frag;
     constexpr int C = Y::KW, NT = C / 16, TT = Y::TT, V = Y::VPL;
     constexpr int KS = DKP / Y::KW, VS = DVS / Y::KW, NI = DKP / 16, NJ = DVS / 16;
+    // bf16 heads of 128, and ragged ones of 64: the weights within a chunk are worked out again for each.  Held, they go to scratch memory,
+    // and a wait for one that comes back is a wait for the next chunk's loads, too (64 x 1024 x 16 heads of 128: 375 us, 308 so; 128 x 1024 x
+    // 16 heads of 60: 351 and 317; whole ones of 64 find room: training, 64 x 512 x 16, 190 and 197)
+    constexpr bool AGAIN = TT == 2 && !STATE_ONLY && (DKP == 128 || (!WHOLE && DKP * DVS >= 4096));
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
     unsigned grp;
@@ -245,16 +249,19 @@ void seq_scan_kernel(const Args A) {
 
     // ---- weights that depend on the head alone, and those that depend on the chunk's length
     float dw[NT][TT][4], wy[V], rx[NT], gn = 1.f;
+    auto within = [&](int g, int m) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int t = 0; t < TT; ++t)
+            for (int t = 0; t < TT; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int x = 16 * nt + m, y = V * g + 4 * t + r, d = rev ? y - x : x - y;
-                const float w = S.a_intra * power(lg, d);
-                dw[nt][t][r] = d >= 0 ? w : 0.f;
-            }
+                for (int r = 0; r < 4; ++r) {
+                    const int x = 16 * nt + m, y = V * g + 4 * t + r, d = rev ? y - x : x - y;
+                    const float w = S.a_intra * power(lg, d);
+                    dw[nt][t][r] = d >= 0 ? w : 0.f;
+                }
+    };
+    if constexpr (!AGAIN) within(g, m);
     int n_have = 0;
     auto by_length = [&](int n) {
         if (n == n_have) return;
@@ -447,6 +454,7 @@ void seq_scan_kernel(const Args A) {
                     for (int nt = 0; nt < NT; ++nt) at[nt][t] = Y::mfma(k, q[nt], at[nt][t]);
                 }
             }
+            if constexpr (AGAIN) within(here(lane) >> 4, here(lane) & 15);
             if (mask) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
