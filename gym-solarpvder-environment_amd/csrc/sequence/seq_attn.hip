@@ -19,7 +19,7 @@
 // eighth of the rate: 20 operations per byte of the 30 at which it turns over.
 //
 // Measured, time of the kernels and share of 5.2 TB/s for each tensor once: forward 128 windows of 2048 tokens x 16 heads of 64,
-// bf16, 489 us, 85 %; 1024 tokens, fp32, 478 us, 86 %; heads of 128, bf16, 64 x 1024 x 16, 308 us, 67 % (the state fills the
+// bf16, 489 us, 85 %; 1024 tokens, fp32, 478 us, 86 %; heads of 128, bf16, 64 x 1024 x 16, 308-346 us, 60-67 % (the state fills the
 // registers and each strip of 32 columns reads Q and K again); heads of 32, 512 x 1024 x 8, 259 us, 80 %.  In pieces: one stream of
 // 16384 tokens x 8 heads of 128, bf16, 94 us, 28 % (states 26, join 18, outputs 50); forward and backward, 4 x 4096 x 16 heads of 64,
 // bf16, 172 us, 30 %.  Windows of 160 x 4 heads of 64, 64 of them, fp32, forward and backward, 61 us, 20 % (latency: ten chunks, one
@@ -165,7 +165,7 @@ void seq_scan_kernel(const Args A) {
     constexpr int C = Y::KW, NT = C / 16, TT = Y::TT, V = Y::VPL;
     constexpr int KS = DKP / Y::KW, VS = DVS / Y::KW, NI = DKP / 16, NJ = DVS / 16;
     // bf16 heads of 128, and ragged ones of 64: the weights within a chunk are worked out again for each.  Held, they go to scratch memory,
-    // and a wait for one that comes back is a wait for the next chunk's loads, too (64 x 1024 x 16 heads of 128: 375 us, 308 so; 128 x 1024 x
+    // and a wait for one that comes back is a wait for the next chunk's loads, too (64 x 1024 x 16 heads of 128: 375 us, 308-346 so; 128 x 1024 x
     // 16 heads of 60: 351 and 317; whole ones of 64 find room: training, 64 x 512 x 16, 190 and 197)
     constexpr bool AGAIN = TT == 2 && !STATE_ONLY && (DKP == 128 || (!WHOLE && DKP * DVS >= 4096));
     extern __shared__ __attribute__((aligned(16))) char lds[];
