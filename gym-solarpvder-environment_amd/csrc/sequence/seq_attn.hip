@@ -517,11 +517,26 @@ void seq_scan_kernel(const Args A) {
                     t = Y::mfma(vf[j], p[nt], t);
                 }
         }
-        if (n > 1 && __any(z != 0.f || z != z)) {
-            pos = pos0;
-            most = 1;
-            n = 0;                                          // (the next turn only loads)
-            continue;
+        if (__any(z != 0.f || z != z)) {
+            if (n > 1) {
+                pos = pos0;
+                most = 1;
+                n = 0;                                      // (the next turn only loads)
+                continue;
+            }
+            // The token is alone.  What a weight of zero keeps from the state -- in a reverse scan an episode that starts with the token, or a
+            // decay that remembers nothing -- is taken out of both factors of the product.
+            if ((rev && mask) || S.a_write * (rev ? gn : 1.f) == 0.f) {
+                frag none;
+#pragma unroll
+                for (int e = 0; e < V; ++e) none[e] = (T)0.f;
+                wave_sync();
+#pragma unroll
+                for (int i = 0; i < NK; ++i) *(frag *)(ldsK + Y::template at<DKP>(i * RK + rk, pk)) = none;
+                wave_sync();
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) vf[j] = none;
+            }
         }
         if constexpr (!STATE_ONLY) {
             const window ow = window_of(O + (long long)a * S.o_t, (unsigned)(n - 1) * o_t + row_v);

@@ -1,0 +1,73 @@
+"""Values that are not finite at the borders of episodes, weights of zero, and grids past their limits, on the GPU."""
+import pytest
+import torch
+
+import sequence_reference as ref
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.bfloat16]
+BAD = [float("nan"), float("inf"), -float("inf")]
+
+
+@pytest.fixture(scope="module")
+def ops(gpu_device):
+    from gym_PVDER_amd.agents import sequence_ops
+    return sequence_ops
+
+
+def _inputs(B, T, H, DK, DV, dtype, dev, seed=0):
+    g = torch.Generator(device="cpu")
+    g.manual_seed(seed)
+    n = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+    return {"q": n(B, T, H, DK).to(dtype).to(dev), "k": n(B, T, H, DK).to(dtype).to(dev), "v": n(B, T, H, DV).to(dtype).to(dev),
+            "log_decay": torch.linspace(-0.02, -0.3, H).to(dev), "do": n(B, T, H, DV).to(dtype).to(dev),
+            "s0": n(B, H, DK, DV).to(dev), "ds": n(B, H, DK, DV).to(dev), "starts": torch.zeros(B, T, dtype=torch.bool, device=dev)}
+
+
+def _gradients(ops, c, **kw):
+    leaf = {n: c[n].detach().requires_grad_() for n in ("q", "k", "v", "s0")}
+    out, end = ops.decay_attention(leaf["q"], leaf["k"], leaf["v"], c["log_decay"], initial_state=leaf["s0"], starts=c["starts"], output_final_state=True, **kw)
+    got = torch.autograd.grad([out, end], list(leaf.values()), [c["do"], c["ds"]])
+    return {"out": out.detach(), "state": end.detach(), **dict(zip(("dq", "dk", "dv", "ds0"), got))}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,at,DK,DV", [(3, 1, 8, 8), (70, 0, 32, 40), (70, 31, 32, 40), (70, 32, 64, 64), (70, 69, 128, 33), (600, 320, 64, 64), (600, 333, 20, 128)])
+def test_the_first_token_of_an_episode_reaches_no_earlier_one(ops, gpu_device, T, at, DK, DV, dtype):
+    """A gradient goes back to the start of its episode and not behind it, whatever the start's own token holds."""
+    c = _inputs(2, T, 2, DK, DV, dtype, gpu_device)
+    c["starts"][:, at] = True
+    clean = ref.attention(c["q"], c["k"], c["v"], c["log_decay"], DK ** -0.5, c["s0"], c["starts"], None, c["do"], c["ds"])
+    mag = ref.attention(c["q"].abs(), c["k"].abs(), c["v"].abs(), c["log_decay"], DK ** -0.5, c["s0"].abs(), c["starts"], None, c["do"].abs(), c["ds"].abs())
+    tol = ref.attention_bounds(dtype, T, DK, DV, clean, mag)
+    for n in ("q", "k", "v", "do"):
+        for bad in BAD:
+            d = dict(c, **{n: c[n].clone()})
+            d[n][0, at, 0, 3] = bad
+            got = _gradients(ops, d)
+            earlier = {m: (got[m][:, :at], clean[m][:, :at], tol[m][:, :at]) for m in ("out", "dq", "dk", "dv")}
+            earlier["ds0"] = got["ds0"], clean["ds0"], tol["ds0"]
+            for m, (x, r, t) in earlier.items():
+                over = (x.double().cpu() - r).abs() > t
+                assert x.shape == r.shape and not bool(over.any() | torch.isnan(x).any()), (n, bad, m)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T", [1, 40, 600])
+def test_a_head_that_remembers_nothing_passes_nothing_on(ops, gpu_device, T, dtype):
+    """A decay of -inf is a weight of zero between any two tokens: values that are not finite stay in their own token, in both directions."""
+    c = _inputs(1, T, 2, 32, 24, dtype, gpu_device)
+    c["log_decay"] = torch.tensor([-float("inf"), -1000.0], device=gpu_device)
+    at = T // 2
+    clean = _gradients(ops, c)
+    others = torch.arange(T, device=gpu_device) != at
+    for n in ("q", "k", "v", "do"):
+        for bad in BAD:
+            d = dict(c, **{n: c[n].clone()})
+            d[n][0, at, :, 3] = bad
+            got = _gradients(ops, d)
+            for m in ("out", "dq", "dk", "dv"):
+                assert torch.isfinite(got[m][:, others].float()).all(), (n, bad, m)
+            assert torch.equal(got["ds0"], torch.zeros_like(got["ds0"])) and torch.equal(clean["ds0"], got["ds0"])
+            if at < T - 1:
+                assert torch.isfinite(got["state"]).all(), (n, bad)
