@@ -60,7 +60,9 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     Args:
         q, k: [N, H, DK], v: [N, H, DV], float32 or bfloat16, any strides; log_decay, scale: as for the window form.
         state: [N, H, DK, DV] float32, contiguous; must not overlap the other tensors.
-        starts: [N] bool or uint8: an episode starts with this token; the row's state is not read.
+        starts: [N] bool or uint8: an episode starts with this token; nothing of the row's state before it counts.
+
+    As in the window form a decay of zero clears also a state that is not finite.
 
     For acting and evaluation: it has no gradient, and refuses tensors that would ask for one.
     """

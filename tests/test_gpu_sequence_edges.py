@@ -71,3 +71,25 @@ def test_a_head_that_remembers_nothing_passes_nothing_on(ops, gpu_device, T, dty
             assert torch.equal(got["ds0"], torch.zeros_like(got["ds0"])) and torch.equal(clean["ds0"], got["ds0"])
             if at < T - 1:
                 assert torch.isfinite(got["state"]).all(), (n, bad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("DK,DV", [(8, 8), (5, 3), (100, 66)])
+def test_steps_clear_with_a_weight_of_zero_as_windows_do(ops, gpu_device, DK, DV, dtype):
+    """A head that remembers nothing takes no state, finite or not: steps behind a window are the window."""
+    c = _inputs(2, 6, 3, DK, DV, dtype, gpu_device)
+    c["log_decay"] = torch.tensor([-float("inf"), -0.1, -1000.0], device=gpu_device)
+    for bad in BAD:
+        k = c["k"].clone()
+        k[0, 1, (0, 2), 2] = bad                                      # (the head with a memory stays finite)
+        out, end = ops.decay_attention(c["q"], k, c["v"], c["log_decay"], output_final_state=True)
+        state = torch.zeros_like(end)
+        state[:, (0, 2)] = bad
+        steps = torch.stack([ops.decay_attention_step(c["q"][:, t], k[:, t], c["v"][:, t], c["log_decay"], state) for t in range(6)], 1)
+        others = torch.arange(6, device=gpu_device) != 1
+        assert torch.isfinite(state).all() and torch.isfinite(steps[:, others].float()).all() and torch.isfinite(out[:, others].float()).all(), bad
+        # heads without a memory: one product a token, the same in both forms but for the order of a sum over DK and the rounding
+        # of its terms to the inputs' type
+        size = (c["q"].float().abs() * k.float().abs()).sum(-1, keepdim=True) * c["v"].float().abs() * DK ** -0.5
+        tol = ((2 * DK + 8) * ref.U32 + (4 * ref.U16 if dtype == torch.bfloat16 else 0.0)) * size
+        assert ((steps.float() - out.float()).abs() <= tol)[:, others][:, :, (0, 2)].all(), bad
