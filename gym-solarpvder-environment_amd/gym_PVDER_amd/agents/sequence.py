@@ -34,8 +34,8 @@ EPS = 1e-6
 def tokens_of(obs: torch.Tensor, action: torch.Tensor, reward: torch.Tensor, starts: torch.Tensor) -> torch.Tensor:
     """Observations [..., 11], the actions and rewards before them [...] and where episodes start [...] -> tokens [..., 17]; the first
     token of an episode has no action and no reward before it."""
-    before = (~starts.bool()).to(obs.dtype)[..., None]
-    return torch.cat([obs, F.one_hot(action.long(), N_ACT).to(obs.dtype) * before, reward.to(obs.dtype)[..., None] * before], -1)
+    before = torch.cat([F.one_hot(action.long(), N_ACT).to(obs.dtype), reward.to(obs.dtype)[..., None]], -1)
+    return torch.cat([obs, before.masked_fill(starts.bool()[..., None], 0.0)], -1)
 
 
 class SequenceBlock(torch.nn.Module):
@@ -121,7 +121,11 @@ class SequenceQNetwork(torch.nn.Module):
 
 class BatchedSequenceDQNAgent:
     """DQN on :class:`SequenceQNetwork`.  The replay buffer holds whole batched steps, so that a window of any env can be read back;
-    the first ``burn_in`` tokens of a window only fill the memory and are left out of the loss."""
+    the first ``burn_in`` tokens of a window only fill the memory and are left out of the loss.
+
+    The env may be reset, stepped or given other events between two calls of :meth:`collect`.  An env that is no
+    longer where the last call left it starts an episode, and what its last action there would have led to is not known: the reward is
+    stored as NaN, and :meth:`loss` leaves that action out. """
 
     train_spec = {'learning_rate': 1e-3, 'batch_size': 64, 'window': 160, 'burn_in': 16, 'replay_steps': 512, 'gamma': 1.0, 'epsilon_greedy': 0.1,
                   'target_update_period': 1, 'width': 64, 'heads': 4, 'head_dim': 16, 'blocks': 2, 'compute_dtype': torch.float32}
@@ -149,6 +153,9 @@ class BatchedSequenceDQNAgent:
         self.steps_in, self.at = 0, 0                       # steps that the ring holds, and the next one's place
         self.state = self.q_net.init_state(N)
         self.action = torch.zeros(N, dtype=torch.uint8, device=dev)
+        # of the next token: the reward behind that action, and whether an episode starts with it
+        self.reward, self.start = torch.zeros(N, dtype=torch.float32, device=dev), torch.ones(N, dtype=torch.bool, device=dev)
+        self.left = None                                    # where collect left the envs: output block, state, clock
         self.train_step_counter = 0
         self.gen = torch.Generator(device=dev)
         self.gen.manual_seed(seed + 1)
@@ -166,29 +173,39 @@ class BatchedSequenceDQNAgent:
         env = self.env
         assert env.auto_reset, "construct the PVDERVec with auto_reset=True: collection runs across episode ends"
         eps = self.spec['epsilon_greedy'] if epsilon is None else epsilon
-        fresh = env._needs_reset
-        if fresh:
+        if env._needs_reset:
             env.reset()
+        out, state, clock = env.out, env.fstate, env.istate[0]
+        if self.left is None:
+            self.left = out.clone(), state.clone(), clock.clone()
+            self.start.fill_(True)
+        else:
+            bits = torch.int64 if state.dtype == torch.float64 else torch.int32
+            moved = (state.view(bits) != self.left[1].view(bits)).any(0) | (clock != self.left[2])
+            self.reward.masked_fill_(moved & ~self.start, float("nan"))     # (an episode that had ended has its last reward)
+            self.start |= moved
+            out = torch.where(moved, out, self.left[0])     # (a block that ``use_out`` has put there holds no observation yet)
         for _ in range(num_steps):
-            s, first = self.at, fresh or self.steps_in == 0
-            self.buf_obs[s].copy_(env.out[:N_OBS].t())
+            s = self.at
+            self.buf_obs[s].copy_(out[:N_OBS].t())
             self.buf_before[s].copy_(self.action)
-            self.buf_reward[s].copy_(env.out[11])
-            # (an env that finished has been reset in the same launch: its observation is the first of the next episode)
-            if first:
-                self.buf_start[s].fill_(True)
-                fresh = False
-            else:
-                self.buf_start[s].copy_(env.out[12] != 0)
+            self.buf_reward[s].copy_(self.reward)
+            self.buf_start[s].copy_(self.start)
             tokens = tokens_of(self.buf_obs[s], self.buf_before[s], self.buf_reward[s], self.buf_start[s])
             self.action.copy_(self._act(self.q_net.step(tokens, self.state, self.buf_start[s]), eps))
             self.buf_action[s].copy_(self.action)
             env.step(self.action, return_tensors=False)
+            # (an env that finished has been reset in the same launch: its observation is the first of the next episode)
+            out = env.out
+            self.reward.copy_(out[11])
+            self.start.copy_(out[12] != 0)
             self.at = (s + 1) % self.buf_obs.shape[0]
             self.steps_in = min(self.steps_in + 1, self.buf_obs.shape[0])
+        for mine, its in zip(self.left, (out, env.fstate, env.istate[0])):
+            mine.copy_(its)
 
     def sample(self):
-        """``batch_size`` windows of ``window`` + 1 tokens: (tokens, starts, actions, rewards behind the actions)."""
+        """``batch_size`` windows of ``window`` + 1 tokens: (tokens, starts, actions, rewards behind the actions, NaN where not known)."""
         sp, dev = self.spec, self.env.device
         B, T, S = int(sp['batch_size']), int(sp['window']) + 1, self.buf_obs.shape[0]
         if self.steps_in < T:
@@ -202,13 +219,15 @@ class BatchedSequenceDQNAgent:
 
     def loss(self, tokens, starts, actions, rewards) -> torch.Tensor:
         """Mean squared one-step error of the action values over the tokens behind ``burn_in``; the value of an episode's end is its
-        reward."""
+        reward, and an action whose reward is NaN does not count."""
         sp = self.spec
         with torch.no_grad():
             after = self.target(tokens, starts=starts)[:, 1:].max(dim=2).values
             wanted = rewards + sp['gamma'] * torch.where(starts[:, 1:], torch.zeros_like(after), after)
+            known = ~torch.isnan(rewards)
         values = self.q_net(tokens[:, :-1], starts=starts[:, :-1]).gather(2, actions[:, :-1, None].long())[..., 0]
-        return ((values - wanted)[:, sp['burn_in']:] ** 2).mean()
+        off = torch.where(known, values - wanted, torch.zeros_like(values))[:, sp['burn_in']:]
+        return (off ** 2).sum() / known[:, sp['burn_in']:].sum().clamp(min=1)
 
     def train_step(self) -> float:
         loss = self.loss(*self.sample())
@@ -245,11 +264,13 @@ class BatchedSequenceDQNAgent:
         alive = torch.ones(N, dtype=torch.bool, device=dev)
         action, starts = torch.zeros(N, dtype=torch.uint8, device=dev), torch.ones(N, dtype=torch.bool, device=dev)
         eval_env.reset()
+        out = eval_env.out
         for _ in range(steps):
-            tokens = tokens_of(eval_env.out[:N_OBS].t().contiguous(), action, eval_env.out[11], starts)
+            tokens = tokens_of(out[:N_OBS].t().contiguous(), action, out[11], starts)
             action.copy_(self._act(self.q_net.step(tokens, state, starts), 0.0))
             starts.fill_(False)
             eval_env.step(action, return_tensors=False)
-            ret += eval_env.out[11].double() * alive
-            alive &= eval_env.out[12] == 0
+            out = eval_env.out
+            ret += out[11].double() * alive
+            alive &= out[12] == 0
         return {"average_return": float(ret.mean()), "min": float(ret.min()), "max": float(ret.max()), "steps": steps, "returns": ret}
