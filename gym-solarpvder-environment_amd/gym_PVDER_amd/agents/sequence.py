@@ -123,9 +123,9 @@ class BatchedSequenceDQNAgent:
     """DQN on :class:`SequenceQNetwork`.  The replay buffer holds whole batched steps, so that a window of any env can be read back;
     the first ``burn_in`` tokens of a window only fill the memory and are left out of the loss.
 
-    The env may be reset, stepped or given other events between two calls of :meth:`collect`.  An env that is no
+    The env may be reset, stepped, sorted (``sort_lanes``) or given other events between two calls of :meth:`collect`.  An env that is no
     longer where the last call left it starts an episode, and what its last action there would have led to is not known: the reward is
-    stored as NaN, and :meth:`loss` leaves that action out. """
+    stored as NaN, and :meth:`loss` leaves that action out.  Buffers and memory are in the order of the env ids."""
 
     train_spec = {'learning_rate': 1e-3, 'batch_size': 64, 'window': 160, 'burn_in': 16, 'replay_steps': 512, 'gamma': 1.0, 'epsilon_greedy': 0.1,
                   'target_update_period': 1, 'width': 64, 'heads': 4, 'head_dim': 16, 'blocks': 2, 'compute_dtype': torch.float32}
@@ -175,7 +175,7 @@ class BatchedSequenceDQNAgent:
         eps = self.spec['epsilon_greedy'] if epsilon is None else epsilon
         if env._needs_reset:
             env.reset()
-        out, state, clock = env.out, env.fstate, env.istate[0]
+        out, state, clock = (env.to_env_order(t) for t in (env.out, env.fstate, env.istate[0]))
         if self.left is None:
             self.left = out.clone(), state.clone(), clock.clone()
             self.start.fill_(True)
@@ -194,14 +194,14 @@ class BatchedSequenceDQNAgent:
             tokens = tokens_of(self.buf_obs[s], self.buf_before[s], self.buf_reward[s], self.buf_start[s])
             self.action.copy_(self._act(self.q_net.step(tokens, self.state, self.buf_start[s]), eps))
             self.buf_action[s].copy_(self.action)
-            env.step(self.action, return_tensors=False)
+            env.step(env.to_lane_order(self.action) if env.lane_io else self.action, return_tensors=False)
             # (an env that finished has been reset in the same launch: its observation is the first of the next episode)
-            out = env.out
+            out = env.to_env_order(env.out)
             self.reward.copy_(out[11])
             self.start.copy_(out[12] != 0)
             self.at = (s + 1) % self.buf_obs.shape[0]
             self.steps_in = min(self.steps_in + 1, self.buf_obs.shape[0])
-        for mine, its in zip(self.left, (out, env.fstate, env.istate[0])):
+        for mine, its in zip(self.left, (out, env.to_env_order(env.fstate), env.to_env_order(env.istate[0]))):
             mine.copy_(its)
 
     def sample(self):
@@ -264,13 +264,13 @@ class BatchedSequenceDQNAgent:
         alive = torch.ones(N, dtype=torch.bool, device=dev)
         action, starts = torch.zeros(N, dtype=torch.uint8, device=dev), torch.ones(N, dtype=torch.bool, device=dev)
         eval_env.reset()
-        out = eval_env.out
+        out = eval_env.to_env_order(eval_env.out)
         for _ in range(steps):
             tokens = tokens_of(out[:N_OBS].t().contiguous(), action, out[11], starts)
             action.copy_(self._act(self.q_net.step(tokens, state, starts), 0.0))
             starts.fill_(False)
-            eval_env.step(action, return_tensors=False)
-            out = eval_env.out
+            eval_env.step(eval_env.to_lane_order(action) if eval_env.lane_io else action, return_tensors=False)
+            out = eval_env.to_env_order(eval_env.out)
             ret += out[11].double() * alive
             alive &= out[12] == 0
         return {"average_return": float(ret.mean()), "min": float(ret.min()), "max": float(ret.max()), "steps": steps, "returns": ret}

@@ -1,4 +1,4 @@
-"""BatchedSequenceDQNAgent on an env that is reset or stepped between two calls of collect."""
+"""BatchedSequenceDQNAgent on an env that is reset, stepped or sorted between two calls of collect."""
 import pytest
 import torch
 
@@ -84,6 +84,40 @@ def test_steps_taken_elsewhere_and_another_output_block(gpu_device):
     env.step(torch.ones(N, dtype=torch.uint8, device=gpu_device))
     agent.collect(2, epsilon=1.0)
     assert agent.buf_start[8].all() and torch.isnan(agent.buf_reward[8]).all()
+
+
+@pytest.mark.parametrize("lane_io", [False, True])
+def test_sorted_lanes_change_no_evaluation(gpu_device, lane_io):
+    from gym_PVDER_amd.vec_env import PVDERVec
+    _, agent = _agent(gpu_device)
+    returns = []
+    for sort in (False, True):
+        env = PVDERVec(N, device=gpu_device, n_sim_time_steps_per_env_step=15, max_sim_time=6.0, seed=5, auto_reset=False)
+        env.reset()
+        if sort:
+            env.sort_lanes(key=torch.arange(N, 0, -1), lane_io=lane_io)
+        returns.append(agent.evaluate(env)["returns"])
+    assert torch.equal(*returns) and len(set(returns[0].tolist())) > 1
+
+
+@pytest.mark.parametrize("lane_io", [False, True])
+def test_sorted_lanes_change_nothing(gpu_device, lane_io):
+    agents = []
+    for sort in (False, True):
+        env, agent = _agent(gpu_device)
+        agent.collect(5, epsilon=0.5)
+        env.reset(torch.arange(N, device=gpu_device) % 5 == 2)
+        agent.collect(5, epsilon=0.5)
+        if sort:
+            env.sort_lanes(lane_io=lane_io)
+            assert not torch.equal(env.env_of_lane.long(), torch.arange(N, device=gpu_device))
+        agent.collect(25, epsilon=0.5)                                           # past ends of episodes
+        agents.append(agent)
+    a, b = agents
+    for n in ("buf_obs", "buf_before", "buf_action", "buf_start"):
+        assert torch.equal(getattr(a, n), getattr(b, n)), n
+    assert torch.equal(torch.nan_to_num(a.buf_reward, 5.0), torch.nan_to_num(b.buf_reward, 5.0))
+    assert all(torch.equal(x, y) for x, y in zip(a.state, b.state))
 
 
 def test_the_loss_leaves_out_what_is_not_known(gpu_device):
