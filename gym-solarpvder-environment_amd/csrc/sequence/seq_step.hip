@@ -30,8 +30,9 @@ template <typename T, int W, int CL, int WAVES> __global__ __launch_bounds__(kBl
     const T *v = (const T *)a.v + n * a.v_n + h * a.v_h;
     T *o = (T *)a.o + n * a.o_n + h * a.o_h;
     float *S = a.state + cell * ((long long)a.dk * a.dv);
+    const uint8_t start = a.starts ? a.starts[n * a.starts_n] : 0;
     const float g = power(log2_decay(a.log_decay[h]), 1);
-    const bool fresh = g == 0.f || (a.starts && a.starts[n * a.starts_n] != 0);    // (a weight of zero clears what is not finite, too)
+    const bool fresh = (start != 0) | (g == 0.f);          // (a weight of zero clears what is not finite, too)
     for (int c0 = 0; c0 < a.dv; c0 += CL * W) {
         const int c = c0 + cl * W;
         const bool in = c < a.dv;                          // (W = 4 only where dv is a multiple of 4)
