@@ -736,6 +736,29 @@ bool fours(const pvder_seq_attn &a, unsigned n_groups, int dkp) {
     return shared && n_groups >= 256;
 }
 
+long long scan_blocks(long long n_groups, unsigned together_log2, int n_sib) {
+    const long long deal = 8ll << together_log2;
+    return (n_groups + deal - 1) / deal * deal * n_sib;
+}
+long long join_items(const pvder_seq_attn &a, int n_sib, int dkp, int dvs) { return (long long)a.B * a.H * n_sib * (dkp * dvs / 4); }
+
+// Whether the threads of each launch that a call with `rows` batch rows makes can be counted
+bool countable(const pvder_seq_attn *a, int rows) {
+    const long long n = (long long)rows * a->H;
+    if (n > kMostThreads || n * a->segments > kMostThreads) return false;
+    pvder_seq_attn all = *a, sub;
+    all.B = rows;
+    int which[PVDER_SEQ_MAX_SCANS];
+    for (const bool first : {true, false})
+        for (const int dkp : {32, 64, 128}) {
+            if ((first && a->segments < 2) || !of_size(&all, dkp, first, sub, which)) continue;
+            const Plan P = plan_of(&sub, dkp);
+            if (scan_blocks(n * a->segments, 2, P.n_sib) > kMostThreads / 64) return false;
+            if (first && join_items(sub, P.n_sib, P.dkp, P.dvs) > kMostThreads - 255) return false;
+        }
+    return true;
+}
+
 int64_t workspace_of(const pvder_seq_attn *a, const Plan &P) {
     const int64_t bhs = (int64_t)a->B * a->H * a->segments;
     return (bhs * P.n_sib * P.dkp * P.dvs + bhs * a->n_scans + 3) / 4 * 4;      // (whole 16 bytes: the next size's begins there)
@@ -756,13 +779,10 @@ States states_of(const float *at, const Plan &P, int scan, int dv, bool transpos
 // `states`: what each piece adds to the state and from that the states that come into the pieces; else the outputs
 template <typename T, int DKP, int DVS, bool WHOLE> int launch(const Args &A, bool states, hipStream_t st) {
     constexpr int MOST = sizeof(T) == 2 ? 3 : 1, LEAST = sizeof(T) == 2 ? 2 : 1;
-    const long long deal = 8ll << A.together_log2, blocks = (A.n_groups + deal - 1) / deal * deal * A.n_sib;
-    if (blocks > 0x7fffffffll) return kEinval;
-    const dim3 grid((unsigned)blocks), block(64);
+    const dim3 grid((unsigned)scan_blocks(A.n_groups, A.together_log2, A.n_sib)), block(64);
     const int bytes = tile_bytes<T>(DKP, DVS);
     if (states) {
-        const long long items = (long long)A.a.B * A.a.H * A.n_sib * (DKP * DVS / 4);
-        if (items / 256 >= 0x7fffffffll) return kEinval;
+        const long long items = join_items(A.a, A.n_sib, DKP, DVS);
         seq_scan_kernel<T, DKP, DVS, WHOLE, true, MOST><<<grid, block, bytes, st>>>(A);
         seq_join_kernel<T, DKP, DVS><<<dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st>>>(A);
     } else {
@@ -790,60 +810,8 @@ template <typename T> int pick(const Args &A, const Plan &P, bool states, hipStr
     return P.dvs == 32 ? fit<T, 128, 32>(A, states, st) : fit<T, 128, NARROW>(A, states, st);
 }
 
-}  // namespace
-
-extern "C" int64_t pvder_seq_attn_plan(pvder_seq_attn *a) {
-    if (!valid(a)) return kEinval;
-    pvder_seq_attn sub;
-    int which[PVDER_SEQ_MAX_SCANS];
-    bool given = false;
-    for (int i = 0; i < a->n_scans; ++i) given = given || a->scan[i].kept;
-    if (given && a->segments < 2) return kEinval;
-    // Pieces of T side by side cost a second reading of K and V, a state of each piece in memory and two more launches: worth it where
-    // the waves leave most of the card idle and the pieces make up for it.  Measured at heads of 64, bf16, one piece against the rule's:
-    // 16 waves of 2048 tokens 82 us and 22 (32 pieces), 128 waves 84 and 35 (8); 512 waves 86 and 100 (4), 1024 waves of 512 61 and 86 (2).
-    // With states that are there already pieces pay up to twice as many waves: forward and backward, 768 waves of 2048 tokens in the
-    // backward pass 262 us in one piece and 236 (fp32), 155 and 157 (bf16), 1152 waves of 1024 110 and 122.
-    long long waves = 0;
-    for (const int dkp : {32, 64, 128})
-        if (of_size(a, dkp, false, sub, which)) waves += (long long)a->B * a->H * plan_of(&sub, dkp).n_sib;
-    if (given) {
-        if (waves > 768) a->segments = 1;
-    } else {
-        a->segments = 1;
-        if (waves >= 1 && waves <= 384 && a->T >= 384) {
-            const long long want = 2048 / waves, most = a->T / 64, n = want < most ? want : most;
-            if (n >= 4) a->segments = (int32_t)n;
-        }
-    }
-    if (a->segments == 1) return 0;
-    int64_t floats = 0;
-    for (const int dkp : {32, 64, 128})
-        if (of_size(a, dkp, true, sub, which)) floats += workspace_of(&sub, plan_of(&sub, dkp));
-    return floats;
-}
-
-extern "C" int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream) {
-    if (!valid(a) || a->segments < 1 || !a->log_decay) return kEinval;
-    if ((long long)a->B * a->H * a->segments > 0x7fffffffll) return kEinval;
-    bool work_needed = false;
-    for (int i = 0; i < a->n_scans; ++i) work_needed = work_needed || (a->segments > 1 && owns(a->scan[i]));
-    if (work_needed && (!a->workspace || ((uintptr_t)a->workspace & 15))) return kEinval;
-    if (a->B > 0 && a->T > 0) {
-        const int64_t most = PVDER_SEQ_MAX_TOKEN_STRIDE / (a->dtype == PVDER_SEQ_BF16 ? 2 : 4);
-        for (int i = 0; i < a->n_scans; ++i) {
-            const pvder_seq_scan &s = a->scan[i];
-            if (!s.q || !s.k || !s.v || !s.o) return kEinval;
-            if ((s.s_in || s.s_out) && (s.s_k < 0 || s.s_v < 0 || s.s_k >= (1ll << 29) || s.s_v >= (1ll << 29) || s.dk * s.s_k + s.dv * s.s_v >= (1ll << 29))) return kEinval;
-            // (a row's end, where the window of a chunk ends, has to lie before the next row)
-            if (s.q_t < s.dk || s.k_t < s.dk || s.v_t < s.dv || s.o_t < s.dv || s.q_t > most || s.k_t > most || s.v_t > most || s.o_t > most) return kEinval;
-            if (s.transpose_of) {
-                const pvder_seq_scan &of = a->scan[s.transpose_of - 1];
-                if (s.k != of.v || s.v != of.k || s.reverse != of.reverse || s.a_write != of.a_write) return kEinval;
-            }
-        }
-    }
-    if (a->B == 0) return 0;
+// All launches of a call whose arguments have been checked
+int run_rows(const pvder_seq_attn *a, hipStream_t st) {
     Args A = {};
     const bool pieces = a->segments > 1 && a->T > 0;
     States states[PVDER_SEQ_MAX_SCANS];
@@ -883,9 +851,89 @@ extern "C" int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream) {
                     }
                 }
             }
-            const int rc = a->dtype == PVDER_SEQ_BF16 ? pick<__bf16>(A, P, first, (hipStream_t)stream) : pick<float>(A, P, first, (hipStream_t)stream);
+            const int rc = a->dtype == PVDER_SEQ_BF16 ? pick<__bf16>(A, P, first, st) : pick<float>(A, P, first, st);
             if (rc) return rc;
         }
+    }
+    return 0;
+}
+
+}  // namespace
+
+extern "C" int64_t pvder_seq_attn_plan(pvder_seq_attn *a) {
+    if (!valid(a)) return kEinval;
+    pvder_seq_attn sub;
+    int which[PVDER_SEQ_MAX_SCANS];
+    bool given = false;
+    for (int i = 0; i < a->n_scans; ++i) given = given || a->scan[i].kept;
+    if (given && a->segments < 2) return kEinval;
+    // Pieces of T side by side cost a second reading of K and V, a state of each piece in memory and two more launches: worth it where
+    // the waves leave most of the card idle and the pieces make up for it.  Measured at heads of 64, bf16, one piece against the rule's:
+    // 16 waves of 2048 tokens 82 us and 22 (32 pieces), 128 waves 84 and 35 (8); 512 waves 86 and 100 (4), 1024 waves of 512 61 and 86 (2).
+    // With states that are there already pieces pay up to twice as many waves: forward and backward, 768 waves of 2048 tokens in the
+    // backward pass 262 us in one piece and 236 (fp32), 155 and 157 (bf16), 1152 waves of 1024 110 and 122.
+    long long waves = 0;
+    for (const int dkp : {32, 64, 128})
+        if (of_size(a, dkp, false, sub, which)) waves += (long long)a->B * a->H * plan_of(&sub, dkp).n_sib;
+    if (given) {
+        if (waves > 768) a->segments = 1;
+    } else {
+        a->segments = 1;
+        if (waves >= 1 && waves <= 384 && a->T >= 384) {
+            const long long want = 2048 / waves, most = a->T / 64, n = want < most ? want : most;
+            if (n >= 4) a->segments = (int32_t)n;
+        }
+    }
+    if (a->segments == 1) return 0;
+    int64_t floats = 0;
+    for (const int dkp : {32, 64, 128})
+        if (of_size(a, dkp, true, sub, which)) floats += workspace_of(&sub, plan_of(&sub, dkp));
+    return floats;
+}
+
+extern "C" int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream) {
+    if (!valid(a) || a->segments < 1 || !a->log_decay) return kEinval;
+    bool work_needed = false;
+    for (int i = 0; i < a->n_scans; ++i) work_needed = work_needed || (a->segments > 1 && owns(a->scan[i]));
+    if (work_needed && (!a->workspace || ((uintptr_t)a->workspace & 15))) return kEinval;
+    if (a->B > 0 && a->T > 0) {
+        const int64_t most = PVDER_SEQ_MAX_TOKEN_STRIDE / (a->dtype == PVDER_SEQ_BF16 ? 2 : 4);
+        for (int i = 0; i < a->n_scans; ++i) {
+            const pvder_seq_scan &s = a->scan[i];
+            if (!s.q || !s.k || !s.v || !s.o) return kEinval;
+            if ((s.s_in || s.s_out) && (s.s_k < 0 || s.s_v < 0 || s.s_k >= (1ll << 29) || s.s_v >= (1ll << 29) || s.dk * s.s_k + s.dv * s.s_v >= (1ll << 29))) return kEinval;
+            // (a row's end, where the window of a chunk ends, has to lie before the next row)
+            if (s.q_t < s.dk || s.k_t < s.dk || s.v_t < s.dv || s.o_t < s.dv || s.q_t > most || s.k_t > most || s.v_t > most || s.o_t > most) return kEinval;
+            if (s.transpose_of) {
+                const pvder_seq_scan &of = a->scan[s.transpose_of - 1];
+                if (s.k != of.v || s.v != of.k || s.reverse != of.reverse || s.a_write != of.a_write) return kEinval;
+            }
+        }
+    }
+    if (a->B == 0) return 0;
+    // as many batch rows at once as the threads of a launch can be counted for (few rows of few heads, where T is in pieces)
+    int rows = a->B;
+    while (!countable(a, rows)) {
+        if (rows == 1 || (a->segments > 1 && a->T > 0)) return kEinval;
+        rows -= rows / 2;
+    }
+    const long long es = a->dtype == PVDER_SEQ_BF16 ? 2 : 4;
+    for (long long b = 0; b < a->B; b += rows) {
+        pvder_seq_attn part = *a;
+        part.B = (int32_t)(a->B - b < rows ? a->B - b : rows);
+        for (int i = 0; i < a->n_scans; ++i) {
+            pvder_seq_scan &s = part.scan[i];
+            s.q = (const char *)s.q + b * s.q_b * es;
+            s.k = (const char *)s.k + b * s.k_b * es;
+            s.v = (const char *)s.v + b * s.v_b * es;
+            s.o = (char *)s.o + b * s.o_b * es;
+            if (s.s_in) s.s_in += b * s.s_b;
+            if (s.s_out) s.s_out += b * s.s_b;
+        }
+        if (a->starts) part.starts = a->starts + b * a->starts_b;
+        if (a->lengths) part.lengths = a->lengths + b;
+        const int rc = run_rows(&part, (hipStream_t)stream);
+        if (rc) return rc;
     }
     return 0;
 }

@@ -8,6 +8,7 @@
 namespace pvder_seq {
 
 constexpr int kEinval = -10001;            // PVDER_EINVAL (pvder_hip.h)
+constexpr long long kMostThreads = 0xffffffffll;           // of a launch: HIP counts them in 32 bits
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f8 __attribute__((ext_vector_type(8)));

@@ -81,13 +81,12 @@ template <typename T, int W, int CL, int WAVES> __global__ __launch_bounds__(kBl
     }
 }
 
+// a large cell is shared by the four waves of a block: one wave would read it in dk / 2 dependent rounds
+bool shared(const pvder_seq_step &a) { return (long long)a.dk * a.dv > 4096; }
+
 template <typename T, int W, int CL> int launch(const pvder_seq_step &a, hipStream_t st) {
-    const long long cells = (long long)a.N * a.H;
-    // a large cell is shared by the four waves of a block: one wave would read it in dk / 2 dependent rounds
-    const bool shared = (long long)a.dk * a.dv > 4096;
-    const long long blocks = shared ? cells : (cells + kBlock / 64 - 1) / (kBlock / 64);
-    if (blocks > 0x7fffffffll) return kEinval;
-    if (shared) seq_step_kernel<T, W, CL, kBlock / 64><<<dim3((unsigned)blocks), dim3(kBlock), 0, st>>>(a);
+    const long long cells = (long long)a.N * a.H, blocks = shared(a) ? cells : (cells + kBlock / 64 - 1) / (kBlock / 64);
+    if (shared(a)) seq_step_kernel<T, W, CL, kBlock / 64><<<dim3((unsigned)blocks), dim3(kBlock), 0, st>>>(a);
     else seq_step_kernel<T, W, CL, 1><<<dim3((unsigned)blocks), dim3(kBlock), 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : -(int)e;
@@ -112,5 +111,21 @@ extern "C" int pvder_seq_step_run(const pvder_seq_step *a, void *stream) {
     if (a->dtype != PVDER_SEQ_F32 && a->dtype != PVDER_SEQ_BF16) return kEinval;
     if (a->N == 0) return 0;
     if (!a->q || !a->k || !a->v || !a->o || !a->state || !a->log_decay) return kEinval;
-    return a->dtype == PVDER_SEQ_BF16 ? pick<__bf16>(*a, (hipStream_t)stream) : pick<float>(*a, (hipStream_t)stream);
+    // as many rows to a launch as its threads can be counted for
+    const long long most = kMostThreads / kBlock * (shared(*a) ? 1 : kBlock / 64) / a->H;
+    if (most < 1) return kEinval;
+    const long long es = a->dtype == PVDER_SEQ_BF16 ? 2 : 4;
+    for (long long n = 0; n < a->N; n += most) {
+        pvder_seq_step part = *a;
+        part.N = (int32_t)(a->N - n < most ? a->N - n : most);
+        part.q = (const char *)a->q + n * a->q_n * es;
+        part.k = (const char *)a->k + n * a->k_n * es;
+        part.v = (const char *)a->v + n * a->v_n * es;
+        part.o = (char *)a->o + n * a->o_n * es;
+        part.state = a->state + n * a->H * ((long long)a->dk * a->dv);
+        if (a->starts) part.starts = a->starts + n * a->starts_n;
+        const int rc = a->dtype == PVDER_SEQ_BF16 ? pick<__bf16>(part, (hipStream_t)stream) : pick<float>(part, (hipStream_t)stream);
+        if (rc) return rc;
+    }
+    return 0;
 }

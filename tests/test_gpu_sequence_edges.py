@@ -93,3 +93,44 @@ def test_steps_clear_with_a_weight_of_zero_as_windows_do(ops, gpu_device, DK, DV
         size = (c["q"].float().abs() * k.float().abs()).sum(-1, keepdim=True) * c["v"].float().abs() * DK ** -0.5
         tol = ((2 * DK + 8) * ref.U32 + (4 * ref.U16 if dtype == torch.bfloat16 else 0.0)) * size
         assert ((steps.float() - out.float()).abs() <= tol)[:, others][:, :, (0, 2)].all(), bad
+
+
+def _far_rows(n, dev):
+    """The first rows, the last ones, and those around the borders of any two or three equal parts."""
+    at = [0, n - 1] + [n * i // p + d for p in (2, 3, 4) for i in range(1, p) for d in range(-40, 40)]
+    return torch.tensor(sorted({min(max(i, 0), n - 1) for i in at}), device=dev)
+
+
+def test_more_cells_than_the_threads_of_a_launch(ops, gpu_device):
+    """Steps of over 2^26 cells, whose launch would have over 2^32 threads."""
+    N = 2 ** 26 + 9
+    g = torch.Generator(device=gpu_device)
+    g.manual_seed(1)
+    q, k, v = (torch.randn(N, 1, 1, generator=g, device=gpu_device) for _ in range(3))
+    state = torch.randn(N, 1, 1, 1, generator=g, device=gpu_device)
+    starts = torch.rand(N, generator=g, device=gpu_device) < 0.25
+    decay = torch.full((1,), -0.25, device=gpu_device)
+    want = (state * torch.exp(decay)).masked_fill(starts[:, None, None, None], 0.0) + k[..., None] * v[..., None]
+    size = state.abs() + (k * v).abs()[..., None]
+    out = ops.decay_attention_step(q, k, v, decay, state, starts=starts)
+    # the weight's exponent and exponential, three products and a sum, on either side
+    assert bool(((state - want).abs() <= 12 * ref.U32 * size).all())
+    assert bool(((out - q * want[..., 0]).abs() <= 14 * ref.U32 * q.abs() * size[..., 0]).all())
+
+
+def test_more_rows_than_the_threads_of_a_launch(ops, gpu_device):
+    """Windows of over 2^26 rows, whose launch would have over 2^32 threads: every tensor of the rows behind the first part."""
+    B, D = 2 ** 26 + 40, 4
+    g = torch.Generator(device=gpu_device)
+    g.manual_seed(2)
+    q, k, v = (torch.randn(B, 1, 1, D, generator=g, device=gpu_device) for _ in range(3))
+    s0 = torch.randn(B, 1, D, D, generator=g, device=gpu_device)
+    starts = torch.rand(B, 1, generator=g, device=gpu_device) < 0.25
+    lengths = (torch.rand(B, generator=g, device=gpu_device) < 0.75).to(torch.int32)
+    decay = torch.full((1,), -0.25, device=gpu_device)
+    out, end = ops.decay_attention(q, k, v, decay, initial_state=s0, starts=starts, lengths=lengths, output_final_state=True)
+    assert torch.isfinite(out).all() and torch.isfinite(end).all()
+    assert not out[lengths == 0].any() and torch.equal(end[lengths == 0], s0[lengths == 0])
+    at = _far_rows(B, gpu_device)
+    few, few_end = ops.decay_attention(q[at], k[at], v[at], decay, initial_state=s0[at], starts=starts[at], lengths=lengths[at], output_final_state=True)
+    assert torch.equal(out[at], few) and torch.equal(end[at], few_end)

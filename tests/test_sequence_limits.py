@@ -1,0 +1,27 @@
+"""Limits of the sequence operators' C entries and of what their Python side takes, without a GPU."""
+import ctypes
+import struct
+
+import pytest
+import torch
+
+from test_sequence_ops import ATTN_TAIL, SCAN, STEP
+
+
+def _attn(B=1, T=1, H=1, dk=8, dv=8, segments=1, work=0):
+    row = max(dk, dv)
+    one = SCAN.pack(*([64] * 4), *([0, row, 0] * 4), 0, 0, *([0] * 4), 0, 1.0, 1.0, 1.0, dk, dv, 0, 0)
+    return ctypes.create_string_buffer(one * 3 + ATTN_TAIL.pack(64, 0, 0, work, 0, 0, B, T, H, 1, 0, segments))
+
+
+def test_launches_whose_threads_cannot_be_counted_are_refused():
+    """A launch has fewer than 2^32 threads.  Batch rows are taken in parts, the heads of one row and the pieces of T are not."""
+    from gym_PVDER_amd import _native
+    _native.build_native()
+    L = _native.sequence_lib()
+    for bad in (dict(H=2 ** 26), dict(H=2 ** 25, dv=128), dict(B=3, H=2 ** 27), dict(H=2 ** 31 - 1), dict(B=2 ** 31 - 1, H=2 ** 31 - 1),
+                dict(B=2 ** 20, H=64, T=512, segments=2, work=64), dict(B=1, H=2 ** 21, T=512, dk=128, dv=128, segments=2, work=64)):
+        assert L.pvder_seq_attn_run(_attn(**bad), None) == _native.EINVAL, bad
+    step = lambda N, H, d: STEP.pack(*([64] * 4), *([0] * 8), 64, 64, 0, 0, N, H, d, d, 0, 1.0)  # noqa: E731
+    for N, H, d in ((1, 2 ** 26, 4), (5, 2 ** 24, 128), (2 ** 31 - 1, 2 ** 31 - 1, 1)):
+        assert L.pvder_seq_step_run(step(N, H, d), None) == _native.EINVAL, (N, H, d)
