@@ -892,7 +892,8 @@ extern "C" int64_t pvder_seq_attn_plan(pvder_seq_attn *a) {
 }
 
 extern "C" int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream) {
-    if (!valid(a) || a->segments < 1 || !a->log_decay) return kEinval;
+    // (more pieces than the plan makes would have tokens past 32 bits)
+    if (!valid(a) || a->segments < 1 || (a->segments > 1 && a->segments > a->T / 64) || !a->log_decay) return kEinval;
     bool work_needed = false;
     for (int i = 0; i < a->n_scans; ++i) work_needed = work_needed || (a->segments > 1 && owns(a->scan[i]));
     if (work_needed && (!a->workspace || ((uintptr_t)a->workspace & 15))) return kEinval;

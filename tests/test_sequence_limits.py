@@ -25,3 +25,11 @@ def test_launches_whose_threads_cannot_be_counted_are_refused():
     step = lambda N, H, d: STEP.pack(*([64] * 4), *([0] * 8), 64, 64, 0, 0, N, H, d, d, 0, 1.0)  # noqa: E731
     for N, H, d in ((1, 2 ** 26, 4), (5, 2 ** 24, 128), (2 ** 31 - 1, 2 ** 31 - 1, 1)):
         assert L.pvder_seq_step_run(step(N, H, d), None) == _native.EINVAL, (N, H, d)
+
+
+def test_more_pieces_than_a_plan_makes_are_refused():
+    """A piece is 64 tokens or more; the kernels count tokens in 32 bits."""
+    from gym_PVDER_amd import _native
+    L = _native.sequence_lib()
+    for T, segments in ((2 ** 30, 2 ** 25), (512, 9), (63, 2), (0, 2)):
+        assert L.pvder_seq_attn_run(_attn(T=T, segments=segments, work=64), None) == _native.EINVAL, (T, segments)
