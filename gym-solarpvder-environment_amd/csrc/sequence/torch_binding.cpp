@@ -165,15 +165,19 @@ std::tuple<Tensor, Tensor> attention_forward(const Tensor &q, const Tensor &k, c
 
 // A leaf's gradient accumulator belongs to the stream on which its first graph was recorded, and lives as long as a graph does.  A
 // backward pass that is captured while such a graph of another stream lives would have to wait for that stream, which a capture cannot:
-// torch's engine throws in a thread of its own, and the process ends.  So the forward pass is refused.
-void capturable(const Tensor &t, const char *name) {
-    if (!t.defined() || !t.requires_grad() || t.grad_fn()) return;
+// torch's engine throws in a thread of its own, and the process ends.  So the forward pass is refused, for arguments that are leaves and
+// for views of leaves.  (A leaf behind other operations meets them first: torch's own captures have the same limit.)
+void capturable(const Tensor &arg, const char *name) {
+    if (!arg.defined() || !arg.requires_grad()) return;
+    Tensor t = arg;
+    if (arg.grad_fn() && arg.is_view()) t = arg._base();
+    if (!t.requires_grad() || t.grad_fn()) return;
     const auto acc = torch::autograd::impl::try_get_grad_accumulator(t);
     if (!acc) return;
     const auto own = acc->stream();
     const c10::Stream now = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).unwrap();
-    TORCH_CHECK(!own || *own == now, name, " is a leaf of a graph that lives on another stream: its backward pass cannot be captured. Delete what holds that graph "
-                "(its outputs, its losses) before the capture.");
+    TORCH_CHECK(!own || *own == now, name, " is a leaf, or a view of one, of a graph that lives on another stream: its backward pass cannot be captured. Delete what "
+                "holds that graph (its outputs, its losses) before the capture.");
 }
 bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
 
@@ -261,6 +265,12 @@ py::object decay_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_,
     const float scale = scale_of(scale_, d.DK);
     on_gpu(q_, "q");
     const c10::DeviceGuard guard(q_.device());
+    if (at::GradMode::is_enabled() && capturing()) {       // (before anything is made of the arguments)
+        capturable(q_, "q");
+        capturable(k_, "k");
+        capturable(v_, "v");
+        if (has(initial_)) capturable(*initial_, "initial_state");
+    }
     const int64_t least = 16 / (int64_t)q_.element_size();
     if (d.DK < least || d.DV < least) {
         // heads of less than 16 bytes: with zeros behind them, and without them again
@@ -278,12 +288,6 @@ py::object decay_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_,
     const optional<Tensor> initial = has(initial_) ? optional<Tensor>(dense(*initial_)) : optional<Tensor>();
     Tensor out, final;
     if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v) || wants_grad(initial))) {
-        if (capturing()) {
-            capturable(q_, "q");
-            capturable(k_, "k");
-            capturable(v_, "v");
-            if (has(initial_)) capturable(*initial_, "initial_state");
-        }
         const auto r = DecayAttention::apply(q, k, v, log_decay, initial, starts, lengths, (double)scale, want_state);
         out = r[0];
         if (want_state) final = r[1];

@@ -134,3 +134,51 @@ def test_more_rows_than_the_threads_of_a_launch(ops, gpu_device):
     at = _far_rows(B, gpu_device)
     few, few_end = ops.decay_attention(q[at], k[at], v[at], decay, initial_state=s0[at], starts=starts[at], lengths=lengths[at], output_final_state=True)
     assert torch.equal(out[at], few) and torch.equal(end[at], few_end)
+
+
+def _inputs_of_a_capture(ops, which, dev):
+    """(the leaf, its operator's outputs as a function of it): a packed leaf's views, heads that are padded, a state."""
+    g = torch.Generator(device="cpu")
+    g.manual_seed(3)
+    n = lambda *s: torch.randn(s, generator=g).to(dev)  # noqa: E731
+    decay = torch.full((2,), -0.1, device=dev)
+    if which == "views of a packed leaf":
+        leaf = n(1, 9, 48).requires_grad_()
+        return leaf, lambda: ops.decay_attention(*(leaf[..., i:i + 16].unflatten(-1, (2, 8)) for i in (0, 16, 32)), decay)
+    if which == "small heads":
+        leaf, k, v = n(1, 9, 2, 3).requires_grad_(), n(1, 9, 2, 3), n(1, 9, 2, 5)
+        return leaf, lambda: ops.decay_attention(leaf, k, v, decay)
+    if which == "small heads, the state":
+        leaf, q, v = n(1, 2, 8, 3).requires_grad_(), n(1, 9, 2, 8), n(1, 9, 2, 3)
+        return leaf, lambda: ops.decay_attention(q, q, v, decay, initial_state=leaf)
+    leaf, y, w = n(4, 3, 8).requires_grad_(), n(12, 8), torch.ones(8, device=dev)
+    return leaf, lambda: ops.gated_residual_norm(y, leaf.view(12, 8), w, w)[1]
+
+
+@pytest.mark.parametrize("which", ["views of a packed leaf", "small heads", "small heads, the state", "a view in the norm"])
+def test_a_capture_beside_a_living_graph_is_refused_behind_views_and_padding(ops, gpu_device, which):
+    """Only forward passes are captured beside the living graph; behind its end forward and backward are, and replay right."""
+    leaf, f = _inputs_of_a_capture(ops, which, gpu_device)
+    out = f()
+    do = torch.randn(out.shape, generator=torch.Generator().manual_seed(4)).to(gpu_device)
+    torch.cuda.synchronize()
+    g, t = torch.cuda.CUDAGraph(), torch.ones(4, device=gpu_device)
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="another stream"):
+            f()
+        with torch.no_grad():
+            quiet = f()                                               # (asks for no gradient)
+        t.mul_(2)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(quiet, out.detach())
+    want = torch.autograd.grad(out, leaf, do)[0].clone()
+    del out
+    g2 = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g2):
+        got = torch.autograd.grad(f(), leaf, do)[0]
+    for _ in range(3):
+        g2.replay()
+        t.add_(1)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
