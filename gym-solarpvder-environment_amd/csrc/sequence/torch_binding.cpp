@@ -4,10 +4,13 @@
 // of one env took 19 us from call to call, 5 here; a training pass over 64 windows of 160 steps 160 us, 60 here, which is its kernels' time.
 #include <torch/extension.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <optional>
 
 #include "pvder_sequence.h"
@@ -42,6 +45,23 @@ void same_device(const Tensor &q, Maybe t, const char *name) {
 void on_gpu(const Tensor &t, const char *name) {
     NEED(t.is_cuda(), name, " is on ", t.device(), ": the kernels need a GPU, there is no CPU path");
 }
+// The kernels take memory, past torch's dispatcher: what it would do to a call besides computing it does not happen.  A tangent would be
+// lost, which torch reads as a derivative of zero; a trace would record outputs that nothing writes.  Both are refused, and so are
+// tensors that stand for others (torch.func, tensor subclasses).  A null is an argument that was not given.
+void plain(std::initializer_list<const Tensor *> all) {
+    NEED(!torch::jit::tracer::isTracing(), "the sequence operators cannot be traced (torch.jit.trace)");
+    typedef c10::impl::TorchDispatchModeKey Mode;
+    for (const Mode m : {Mode::FAKE, Mode::PROXY, Mode::FUNCTIONAL})
+        NEED(!c10::impl::TorchDispatchModeTLS::get_mode(m).has_value(), "the sequence operators cannot be traced (make_fx, fake tensors)");
+    for (const Tensor *t : all) {
+        if (!t || !t->defined()) continue;
+        NEED(t->has_storage() && !t->key_set().has(c10::DispatchKey::Python) && !t->key_set().has(c10::DispatchKey::Functionalize),
+             "the sequence operators take plain tensors, not wrappers of them (torch.func, tensor subclasses with __torch_dispatch__)");
+        NEED(!t->_fw_grad(0).defined(), "the sequence operators have no forward-mode gradient: an argument has a tangent");
+    }
+}
+const Tensor *given(Maybe t) { return has(t) ? &*t : nullptr; }
+
 bool wants_grad(const Tensor &t) { return t.requires_grad(); }
 bool wants_grad(Maybe t) { return has(t) && t->requires_grad(); }
 
@@ -247,6 +267,7 @@ struct DecayAttention : torch::autograd::Function<DecayAttention> {
 
 py::object decay_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &log_decay, optional<double> scale_, Maybe initial_,
                            Maybe starts, Maybe lengths, bool want_state) {
+    plain({&q_, &k_, &v_, &log_decay, given(initial_), given(starts), given(lengths)});
     const Heads d = check_qkv(q_, k_, v_, log_decay, 4, "[B, T, H, D]");
     const int64_t B = q_.size(0), T = q_.size(1);
     same_device(q_, initial_, "initial_state");
@@ -300,6 +321,7 @@ py::object decay_attention(const Tensor &q_, const Tensor &k_, const Tensor &v_,
 
 Tensor decay_attention_step(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &log_decay, const Tensor &state, optional<double> scale_,
                             Maybe starts) {
+    plain({&q_, &k_, &v_, &log_decay, &state, given(starts)});
     const Heads d = check_qkv(q_, k_, v_, log_decay, 3, "[N, H, D]");
     const int64_t N = q_.size(0);
     same_device(q_, state, "state");
@@ -416,6 +438,7 @@ struct GatedResidualNorm : torch::autograd::Function<GatedResidualNorm> {
 };
 
 std::tuple<Tensor, Tensor> gated_residual_norm(const Tensor &h, const Tensor &y, const Tensor &post, const Tensor &pre, Maybe gate, Maybe scale, double eps) {
+    plain({&h, &y, &post, &pre, given(gate), given(scale)});
     same_device(h, y, "y");
     same_device(h, post, "post_weight");
     same_device(h, pre, "pre_weight");

@@ -10,7 +10,8 @@ memory.  This one has a fixed size per env, so that 65 536 envs act in one launc
 windows in parallel.  ``agents/sequence.py`` holds the network and the agent that use them.
 
 All calls are asynchronous on the current stream of the inputs' device, can be captured into a HIP graph, and refuse (``ValueError``,
-``TypeError``) what the kernels do not take.  There is no CPU fallback.  Checks, outputs and autograd nodes are in
+``TypeError``) what the kernels do not take: forward-mode tangents, ``torch.func`` transforms, tracing (``torch.jit.trace``, ``make_fx``)
+and tensors that wrap others among it.  There is no CPU fallback.  Checks, outputs and autograd nodes are in
 csrc/sequence/torch_binding.cpp.
 """
 from __future__ import annotations

@@ -182,3 +182,25 @@ def test_a_capture_beside_a_living_graph_is_refused_behind_views_and_padding(ops
         t.add_(1)
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+def test_tangents_are_refused_and_checkpoints_are_not(ops, gpu_device):
+    import torch.autograd.forward_ad as fwad
+    from torch.utils.checkpoint import checkpoint
+    from torch.utils.flop_counter import FlopCounterMode
+    c = _inputs(2, 600, 2, 16, 16, torch.float32, gpu_device)
+    f = lambda q: ops.decay_attention(q, c["k"], c["v"], c["log_decay"], starts=c["starts"])  # noqa: E731
+    with fwad.dual_level(), pytest.raises(ValueError, match="tangent"):
+        f(fwad.make_dual(c["q"], torch.ones_like(c["q"])))
+    q = c["q"].detach().requires_grad_()
+    want, = torch.autograd.grad(f(q), q, c["do"])
+    with FlopCounterMode(display=False):
+        again, = torch.autograd.grad(f(q), q, c["do"])
+    assert torch.equal(again, want)
+    for reentrant in (False, True):
+        q.grad = None
+        checkpoint(f, q, use_reentrant=reentrant).backward(c["do"])
+        assert torch.equal(q.grad, want), reentrant
+    with torch.autograd.graph.save_on_cpu():
+        out = f(q)
+    assert torch.equal(torch.autograd.grad(out, q, c["do"])[0], want)

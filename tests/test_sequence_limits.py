@@ -33,3 +33,54 @@ def test_more_pieces_than_a_plan_makes_are_refused():
     L = _native.sequence_lib()
     for T, segments in ((2 ** 30, 2 ** 25), (512, 9), (63, 2), (0, 2)):
         assert L.pvder_seq_attn_run(_attn(T=T, segments=segments, work=64), None) == _native.EINVAL, (T, segments)
+
+
+def _calls():
+    from gym_PVDER_amd.agents import sequence_ops as so
+    q, g, w, state = torch.zeros(2, 5, 2, 8), torch.zeros(2), torch.ones(8), torch.zeros(5, 2, 8, 8)
+    t, h = q[0], q[0, 0]
+    return {"windows": (lambda x: so.decay_attention(x, q, q, g), q),
+            "the state of windows": (lambda x: so.decay_attention(q, q, q, g, initial_state=x), torch.zeros(2, 2, 8, 8)),
+            "steps": (lambda x: so.decay_attention_step(t, t, x, g, state), t),
+            "the state of steps": (lambda x: so.decay_attention_step(t, t, t, g, x), state),
+            "norm": (lambda x: so.gated_residual_norm(h, x, w, w)[0], h),
+            "a weight of the norm": (lambda x: so.gated_residual_norm(h, h, w, w, scale=x)[0], w)}
+
+
+@pytest.mark.parametrize("name", sorted(_calls()))
+def test_what_the_kernels_would_silently_leave_out_is_refused(name):
+    """A tangent would be dropped, a trace would record memory that nothing writes."""
+    import torch.autograd.forward_ad as fwad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, x = _calls()[name]
+    with pytest.raises(ValueError, match="GPU"):
+        f(x)
+    with fwad.dual_level(), pytest.raises(ValueError, match="tangent"):
+        f(fwad.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(ValueError, match="traced"):
+        torch.jit.trace(f, (x,))
+    for mode in ("real", "fake", "symbolic"):
+        with pytest.raises(ValueError, match="traced"):
+            make_fx(f, tracing_mode=mode)(x)
+    for transform in (lambda: torch.func.jvp(f, (x,), (x,)), lambda: torch.func.vmap(f)(x[None]), lambda: torch.func.functionalize(f)(x),
+                      lambda: torch.func.grad(lambda t: f(t).sum())(x)):
+        with pytest.raises(ValueError, match="traced|wrappers"):
+            transform()
+
+
+class _Logged(torch.Tensor):
+    """A tensor subclass that sees the operations on it."""
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        return func(*args, **(kwargs or {}))
+
+
+def test_tensors_that_stand_for_others_are_refused_and_parameters_are_not():
+    f, x = _calls()["windows"]
+    with pytest.raises(ValueError, match="wrappers"):
+        f(torch.Tensor._make_subclass(_Logged, x))
+    with pytest.raises(ValueError, match="GPU"):
+        f(torch.nn.Parameter(x))
+    from torch.utils.flop_counter import FlopCounterMode
+    with FlopCounterMode(display=False), pytest.raises(ValueError, match="GPU"):     # (counts, and changes nothing)
+        f(x)
