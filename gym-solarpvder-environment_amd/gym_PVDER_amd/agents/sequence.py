@@ -60,8 +60,8 @@ class SequenceQNetwork(torch.nn.Module):
             raise ValueError("compute_dtype must be float32 or bfloat16")
         if min(width, heads, head_dim, blocks) < 1 or head_dim > 128 or width > 8192:
             raise ValueError("width must be in 1..8192, head_dim in 1..128, heads and blocks at least 1")
-        if len(horizons) != 2 or min(horizons) <= 1.0:
-            raise ValueError("horizons are two numbers of env steps above 1")
+        if len(horizons) != 2 or not all(1.0 < x < float("inf") for x in horizons):
+            raise ValueError("horizons are two finite numbers of env steps above 1")
         self.width, self.heads, self.head_dim, self.compute_dtype = int(width), int(heads), int(head_dim), compute_dtype
         self.embed = torch.nn.Parameter(torch.empty(width, N_TOKEN))
         self.embed_bias = torch.nn.Parameter(torch.zeros(width))

@@ -84,3 +84,13 @@ def test_tensors_that_stand_for_others_are_refused_and_parameters_are_not():
     from torch.utils.flop_counter import FlopCounterMode
     with FlopCounterMode(display=False), pytest.raises(ValueError, match="GPU"):     # (counts, and changes nothing)
         f(x)
+
+
+def test_horizons_are_finite():
+    """An infinite one made decays that are not numbers, which the kernels take as none."""
+    from gym_PVDER_amd.agents import SequenceQNetwork
+    for bad in ((4.0, float("inf")), (float("nan"), 5.0), (4.0, float("nan")), (1.0, 5.0), (4.0,)):
+        with pytest.raises(ValueError, match="horizons"):
+            SequenceQNetwork(horizons=bad, device="cpu")
+    decay = SequenceQNetwork(horizons=(4.0, 1e9), device="cpu").log_decay
+    assert torch.isfinite(decay).all() and (decay < 0).all() and bool((decay[1:] > decay[:-1]).all())
