@@ -897,12 +897,15 @@ extern "C" int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream) {
     bool work_needed = false;
     for (int i = 0; i < a->n_scans; ++i) work_needed = work_needed || (a->segments > 1 && owns(a->scan[i]));
     if (work_needed && (!a->workspace || ((uintptr_t)a->workspace & 15))) return kEinval;
+    for (int i = 0; i < a->n_scans; ++i) {                  // (states go in and out also where there is no token)
+        const pvder_seq_scan &s = a->scan[i];
+        if ((s.s_in || s.s_out) && (s.s_k < 0 || s.s_v < 0 || s.s_k >= (1ll << 29) || s.s_v >= (1ll << 29) || s.dk * s.s_k + s.dv * s.s_v >= (1ll << 29))) return kEinval;
+    }
     if (a->B > 0 && a->T > 0) {
         const int64_t most = PVDER_SEQ_MAX_TOKEN_STRIDE / (a->dtype == PVDER_SEQ_BF16 ? 2 : 4);
         for (int i = 0; i < a->n_scans; ++i) {
             const pvder_seq_scan &s = a->scan[i];
             if (!s.q || !s.k || !s.v || !s.o) return kEinval;
-            if ((s.s_in || s.s_out) && (s.s_k < 0 || s.s_v < 0 || s.s_k >= (1ll << 29) || s.s_v >= (1ll << 29) || s.dk * s.s_k + s.dv * s.s_v >= (1ll << 29))) return kEinval;
             // (a row's end, where the window of a chunk ends, has to lie before the next row)
             if (s.q_t < s.dk || s.k_t < s.dk || s.v_t < s.dv || s.o_t < s.dv || s.q_t > most || s.k_t > most || s.v_t > most || s.o_t > most) return kEinval;
             if (s.transpose_of) {

@@ -8,9 +8,9 @@ import torch
 from test_sequence_ops import ATTN_TAIL, SCAN, STEP
 
 
-def _attn(B=1, T=1, H=1, dk=8, dv=8, segments=1, work=0):
+def _attn(B=1, T=1, H=1, dk=8, dv=8, segments=1, work=0, states=(0, 0), state_strides=(0, 0, 0, 0)):
     row = max(dk, dv)
-    one = SCAN.pack(*([64] * 4), *([0, row, 0] * 4), 0, 0, *([0] * 4), 0, 1.0, 1.0, 1.0, dk, dv, 0, 0)
+    one = SCAN.pack(*([64] * 4), *([0, row, 0] * 4), *states, *state_strides, 0, 1.0, 1.0, 1.0, dk, dv, 0, 0)
     return ctypes.create_string_buffer(one * 3 + ATTN_TAIL.pack(64, 0, 0, work, 0, 0, B, T, H, 1, 0, segments))
 
 
@@ -33,6 +33,16 @@ def test_more_pieces_than_a_plan_makes_are_refused():
     L = _native.sequence_lib()
     for T, segments in ((2 ** 30, 2 ** 25), (512, 9), (63, 2), (0, 2)):
         assert L.pvder_seq_attn_run(_attn(T=T, segments=segments, work=64), None) == _native.EINVAL, (T, segments)
+
+
+def test_states_whose_offsets_pass_32_bits_are_refused():
+    """Also those of windows without a token, whose state goes through all the same."""
+    from gym_PVDER_amd import _native
+    L = _native.sequence_lib()
+    for T in (0, 1):
+        for states in ((64, 0), (0, 64)):
+            for strides in ((0, 0, 2 ** 29, 1), (0, 0, 1, 2 ** 29), (0, 0, 2 ** 26, 1), (0, 0, -1, 1), (0, 0, 1, -8)):
+                assert L.pvder_seq_attn_run(_attn(T=T, states=states, state_strides=strides), None) == _native.EINVAL, (T, states, strides)
 
 
 def _calls():
