@@ -14,15 +14,16 @@
 // (`STATE_ONLY`), the states that come into the pieces (seq_join_kernel), and the outputs.  The three gradients are scans too; of
 // their piece states the backward pass works out one, that of dv: dk's is its transpose, dq's the transpose of the forward pass's.
 //
-// Bound: bytes.  A token of a head costs (2 dk + 2 dv) elements and 4 dk dv + 2 C (dk + dv) operations: with bf16, dk = dv = 64
-// and C = 32 that is 48 operations per byte, where the card turns over at about 240.  fp32 has C = 16 and matrix instructions of an
-// eighth of the rate: 20 operations per byte of the 30 at which it turns over.
+// Bound: bytes.  A token of a head costs (2 dk + 2 dv) elements and (2 + 2 p) dk dv + 2 C (dk + dv) operations, p the summands of w V
+// (`weighted`): with bf16, dk = dv = 64 and C = 32 that is 64 operations per byte for p = 2, 80 for p = 3, and 8 more for the check that K
+// and V are finite, where the card turns over at about 240.  fp32 has p = 1, C = 16 and matrix instructions of an eighth of the rate: 20
+// operations per byte of the 30 at which it turns over.
 //
 // Measured, time of the kernels and share of 5.2 TB/s for each tensor once: forward 128 windows of 2048 tokens x 16 heads of 64,
-// bf16, 489 us, 85 %; 1024 tokens, fp32, 478 us, 86 %; heads of 128, bf16, 64 x 1024 x 16, 308-346 us, 60-67 % (the state fills the
-// registers and each strip of 32 columns reads Q and K again); heads of 32, 512 x 1024 x 8, 259 us, 80 %.  In pieces: one stream of
-// 16384 tokens x 8 heads of 128, bf16, 94 us, 28 % (states 26, join 18, outputs 50); forward and backward, 4 x 4096 x 16 heads of 64,
-// bf16, 172 us, 30 %.  Windows of 160 x 4 heads of 64, 64 of them, fp32, forward and backward, 61 us, 20 % (latency: ten chunks, one
+// bf16, 489 us, 85 %; 1024 tokens, fp32, 476 us, 86 %; heads of 128, bf16, 64 x 1024 x 16, 300-316 us, 65-69 % (the state fills the
+// registers and each strip of 32 columns reads Q and K again); heads of 32, 512 x 1024 x 8, 260 us, 79 %.  In pieces: one stream of
+// 16384 tokens x 8 heads of 128, bf16, 96 us, 27 % (states 27, join 18, outputs 51); forward and backward, 4 x 4096 x 16 heads of 64,
+// bf16, 170 us, 31 %.  Windows of 160 x 4 heads of 64, 64 of them, fp32, forward and backward, 61 us, 20 % (latency: ten chunks, one
 // behind the other).
 #include "seq_common.hpp"
 
@@ -73,7 +74,8 @@ template <> struct Ty<__bf16> {
         return __builtin_convertvector(x, b8);
     }
     // w_y v_y as P summands of 8 bits each, P - 1 of them below the first: three are fp32's 24 bits, so a state that is returned is an fp32
-    // sum of fp32 products; two (2^-17 of each term) where only outputs of 8 bits are made of it.  One (2^-9) would show there too.
+    // sum of fp32 products; two (off by 2^-16 of each term at most) where only outputs of 8 bits are made of it.  One (2^-8) would show there
+    // too.
     template <int P> static __device__ __forceinline__ void weighted(frag v, const float *w, frag *part) {
         f8 x = __builtin_convertvector(v, f8);
 #pragma unroll
@@ -484,8 +486,11 @@ void seq_scan_kernel(const Args A) {
         for (int j = 0; j < NJ; ++j) vf[j] = Y::template column<DVS>(ldsV, j, m, g);
         f4 o[VS][NT][TT];
         if constexpr (!STATE_ONLY) {
-            // P and S as operands are rounded to the inputs' type: 2^-9 of each term at bf16, as much as the output's own rounding; the
-            // sums are fp32
+            // P and S as operands are rounded to the inputs' type: 2^-8 of each term at most with bf16, as much as the output's own rounding;
+            // the sums, and the state that goes on, are fp32.  Outputs are off by 0.0023 of their norm then, by 0.0017 with each in two summands
+            // (their own rounding).  That would cost 2 % where the card is full (128 x 2048 x 16 heads of 64: 484 us, 493), 6-9 % on windows and
+            // pieces (96 x 157 x 4: 15.6, 17.1; 16384 x 8 heads of 128: 98, 106), 11-14 % where registers are short (training, 64 x 512 x 16
+            // heads of 64: 227, 252; 64 x 1024 x 16 heads of 128: 301, 343).
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -728,8 +733,8 @@ Plan plan_of(const pvder_seq_attn *a, int dkp) {
 }
 
 // Whether four (b, h, piece) on end go to one XCD: where there are enough to go round, and rows of less than a line share theirs with the
-// next head's (512 x 1024 x 8 heads of 32, bf16: 290 us one by one, 259 by fours, 256 by eights) or heads are of 128 (64 x 1024 x 16: 393,
-// 376, 378).  Else it is no gain: 128 x 2048 x 16 heads of 64 486, 491, 504; 64 windows of 160 x 4 heads of 64, fp32, 61.5, 63, 63.
+// next head's (512 x 1024 x 8 heads of 32, bf16: 290 us one by one, 259 by fours, 256 by eights) or heads are of over 64 (64 x 1024 x 16 of
+// 128: 327, 315, 315; of 100: 499, 476, 467; forward and backward, 32 x 1024 x 16 of 128: 598, 590, 586).  Else it is no gain: 128 x 2048 x 16 heads of 64 486, 491, 504; 64 windows of 160 x 4 heads of 64, fp32, 61.5, 63, 63.
 bool fours(const pvder_seq_attn &a, unsigned n_groups, int dkp) {
     bool shared = dkp == 128 && a.segments == 1;
     for (int i = 0; i < a.n_scans; ++i) shared = shared || (a.scan[i].dk < a.scan[i].dv ? a.scan[i].dk : a.scan[i].dv) * (a.dtype == PVDER_SEQ_BF16 ? 2 : 4) < 128;

@@ -48,8 +48,16 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
 
     Differentiable once in q, k, v and initial_state, through both outputs.  A value that is not finite reaches its own token and the
     later ones of its episode (in a gradient: the earlier ones), as in the recurrence above; an infinity may arrive as NaN.  A weight of
-    zero, which a decay of -inf or one small enough reaches, clears also what is not finite.  For a graph of few, long windows the forward
-    pass keeps up to 33 MB of states besides its inputs.
+    zero, which a decay of -inf, one small enough or a start reaches, clears also what is not finite.
+
+    States and all sums are held in float32.  With bfloat16 inputs the scores and the state are rounded to bfloat16 where they enter the
+    products that make outputs and gradients of that type: an output is off by about 1.4 roundings of its own; float32 inputs have none of
+    this.  A state that is returned (``output_final_state``, the gradient of ``initial_state``) is made of products of 24 bits, else of 16, so
+    the last bits of bfloat16 results can depend on whether it is asked for.  Any call repeated gives the same bits.
+
+    A capture into a HIP graph is refused (``RuntimeError``) where q, k, v or initial_state is a leaf, or a view of one, of a graph that lives
+    on another stream: the backward pass would end the process.  Of few, long windows whose gradients are wanted the forward pass keeps up to
+    33 MB of states besides its inputs.
     """
     return _native.sequence_torch().decay_attention(q, k, v, log_decay, scale, initial_state, starts, lengths, output_final_state)
 
@@ -63,7 +71,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
         state: [N, H, DK, DV] float32, contiguous; must not overlap the other tensors.
         starts: [N] bool or uint8: an episode starts with this token; nothing of the row's state before it counts.
 
-    As in the window form a decay of zero clears also a state that is not finite.
+    As in the window form a weight of zero (a decay of -inf, a start) clears also a state that is not finite.
 
     For acting and evaluation: it has no gradient, and refuses tensors that would ask for one.
     """

@@ -3,7 +3,8 @@
  *
  * Conventions of pvder_hip.h: plain device pointers, a hipStream_t, asynchronous, allocation-free (workspaces come from the
  * caller); 0 / PVDER_EINVAL (-10001) / -hipError_t.  Nothing is launched when a call is refused.  Strides count elements;
- * the last dimension of every tensor has stride 1 unless a field says otherwise.  All offsets are 64-bit. */
+ * the last dimension of every tensor has stride 1 unless a field says otherwise.  All offsets are 64-bit.  A launch has fewer than
+ * 2^32 threads: rows (B, N) beyond that are taken in several launches, heads of one row and pieces of T are refused. */
 #ifndef PVDER_SEQUENCE_H
 #define PVDER_SEQUENCE_H
 #include <stddef.h>
@@ -43,7 +44,7 @@ typedef struct pvder_seq_attn {
     const int32_t *lengths;         /* NULL or [B]: tokens of each row, taken into 0 .. T */
     float *workspace;               /* pvder_seq_attn_plan() floats, 16-byte aligned; NULL when that is 0 */
     int64_t starts_b, starts_t;
-    int32_t B, T, H, n_scans, dtype, segments;   /* segments: as pvder_seq_attn_plan() set it */
+    int32_t B, T, H, n_scans, dtype, segments;   /* segments: as pvder_seq_attn_plan() set it, at most T / 64 */
 } pvder_seq_attn;
 
 /* Sets a->segments, the pieces of T that run side by side, by B, T, H, n_scans, dtype and the scans' dk, dv, kept and transpose_of alone
@@ -57,7 +58,7 @@ typedef struct pvder_seq_attn {
 int64_t pvder_seq_attn_plan(pvder_seq_attn *a);
 int pvder_seq_attn_run(const pvder_seq_attn *a, void *stream);
 
-/* One token of every row n and head h:  S = g S + k v^T (S taken as zeros where starts[n] != 0),  o = scale S^T q.  The state is
+/* One token of every row n and head h:  S = g S + k v^T (S taken as zeros where starts[n] != 0 or g is 0),  o = scale S^T q.  The state is
  * updated in place; `state` is contiguous [N, H, dk, dv]. */
 typedef struct pvder_seq_step {
     const void *q, *k, *v;          /* [N, H, dk], [N, H, dk], [N, H, dv] */
